@@ -260,6 +260,70 @@ typedef struct msr_adamw8bit_hparams {
 int msr_adamw8bit(const msr_adamw8bit_entry* entries, int count, const float* qmap1,
                   const float* qmap2, const msr_adamw8bit_hparams* hp, msr_stream_t stream);
 
+/* ---- Gradient norm and clipping (no counterpart in the reference) -----------------------
+ * Between the backward pass and the step. With p = 1, 2 or infinity over the elements of all
+ * entries together:
+ *   power  = sum |g|^p (the largest |g| for infinity);  norm = scale * power^(1/p)
+ *   coef   = min(1, max_norm / (norm + 1e-6));          factor = scale * coef
+ * `scale` is what the caller multiplies every gradient by in any case (1 / micro-batches, 1 /
+ * loss scale); max_norm = INFINITY asks for coef = 1 whatever the norm. Sums are kept in
+ * double, in a fixed order: the same inputs give the same bits. NaN anywhere gives a NaN norm and
+ * factor; an infinity gives norm = infinity and coef = 0.
+ * msr_grad_norm writes `state` and, where `each` is given, the norm of every entry by itself
+ * (scale included). The workspace is scratch of this call alone; two calls that may overlap
+ * need one each.
+ * msr_grad_factor computes norm, factor and active again from state->power, for a caller that
+ * combined the powers of several ranks (a sum, or for infinity a maximum -- of the bit patterns
+ * as int64 where NaN has to survive it; powers are never negative).
+ * msr_grad_scale multiplies every entry by state->factor in place, in fp32, rounded to nearest
+ * even; when state->active is 0 it leaves them untouched. Entries of one call must not share
+ * memory (MSR_ERR_INVALID). An entry may start at any multiple of its element size; entries of
+ * numel 0 may have a NULL pointer. */
+enum msr_dtype { MSR_BF16 = 0, MSR_FP16 = 1, MSR_FP32 = 2 };
+enum msr_norm { MSR_NORM_INF = 0, MSR_NORM_1 = 1, MSR_NORM_2 = 2 };
+
+typedef struct msr_grad_entry {
+  void* grad;
+  int64_t numel;
+  int32_t dtype;       /* MSR_BF16, MSR_FP16 or MSR_FP32 */
+  int32_t reserved;
+} msr_grad_entry;
+
+typedef struct msr_clip_state {  /* in device memory, 8-byte aligned */
+  double power;
+  float norm;
+  float factor;
+  int32_t active;      /* 0: factor is 1 and there is nothing to scale */
+  int32_t reserved;
+} msr_clip_state;
+
+size_t msr_grad_norm_workspace_bytes(int count);
+
+int msr_grad_norm(const msr_grad_entry* entries, int count, int norm, double scale, double max_norm,
+                  msr_clip_state* state, float* each, void* workspace, size_t workspace_bytes,
+                  msr_stream_t stream);
+
+int msr_grad_factor(msr_clip_state* state, int norm, double scale, double max_norm, msr_stream_t stream);
+
+int msr_grad_scale(const msr_grad_entry* entries, int count, const msr_clip_state* state,
+                   msr_stream_t stream);
+
+/* The updates above with every gradient read as g * grad_factor[0], an fp32 scalar in device
+ * memory (state->factor of msr_grad_norm): the product is taken in fp32 and is not rounded to
+ * bf16, and the gradients themselves stay. Everything else -- noise, order of the operations,
+ * records -- is that of the call without the suffix, and grad_factor[0] = 1 gives its bits. */
+int msr_muon_prepare_scaled(const msr_prepare_entry* entries, int count, float beta, float one_minus_beta,
+                            int nesterov, const float* grad_factor, msr_stream_t stream);
+int msr_adamw_sr_scaled(const msr_adamw_entry* entries, int count, const msr_adamw_hparams* hp,
+                        const float* grad_factor, msr_stream_t stream);
+int msr_muon_prepare_rec_scaled(const msr_prepare_entry* entries, int count, const void* record,
+                                const float* grad_factor, msr_stream_t stream);
+int msr_adamw_sr_rec_scaled(const msr_adamw_entry* entries, int count, const void* record,
+                            const float* grad_factor, msr_stream_t stream);
+int msr_adamw8bit_scaled(const msr_adamw8bit_entry* entries, int count, const float* qmap1,
+                         const float* qmap2, const msr_adamw8bit_hparams* hp, const float* grad_factor,
+                         msr_stream_t stream);
+
 /* ---- Newton-Schulz ---------------------------------------------------------------------
  * out[b] = NS_steps(x[b]) for b < batch, x and out bf16 [batch, rows, cols] contiguous.
  * Quintic iteration (a, b, c) = (3.4445, -4.7750, 2.0315) on the wide orientation

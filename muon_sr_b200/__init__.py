@@ -9,6 +9,7 @@ library ``libmuon_sr_b200.so``. There is no CPU fallback.
 from ._version import __version__
 from .adamw import SRAccumulator, TritonAdamW, TritonSRAccumulator
 from .adamw8bit import TritonAdamW8bit, create_dynamic_map
+from .clipping import clip_grad_norm_, get_total_norm
 from .muon import MuonSR, MuonSRWithAuxAdam, TritonMuonSR, TritonMuonSRWithAuxAdam
 from .kernels import set_sr_noise
 from .sharding import Sharder
@@ -22,4 +23,5 @@ __all__ = [
     "MuonSR", "MuonSRWithAuxAdam",
     "TritonMuonSR", "TritonMuonSRWithAuxAdam",
     "Sharder", "HostStaging", "StepGraph", "create_dynamic_map", "set_sr_noise",
+    "clip_grad_norm_", "get_total_norm",
 ]

@@ -18,6 +18,7 @@ c_int32 = ctypes.c_int32
 c_int64 = ctypes.c_int64
 c_uint64 = ctypes.c_uint64
 c_float = ctypes.c_float
+c_double = ctypes.c_double
 c_size_t = ctypes.c_size_t
 
 
@@ -40,6 +41,16 @@ class AdamWEntry(ctypes.Structure):
 class AdamWHparams(ctypes.Structure):
     _fields_ = [("beta1", c_float), ("one_minus_beta1", c_float), ("beta2", c_float),
                 ("one_minus_beta2", c_float), ("eps", c_float), ("decay", c_float)]
+
+
+# Entries of the gradient norm as int64 triples (msr_grad_entry): pointer, elements, dtype code
+# (the low half of the third word; its high half is the reserved field).
+GRAD_ENTRY_WORDS = 3
+
+
+class ClipState(ctypes.Structure):
+    _fields_ = [("power", c_double), ("norm", c_float), ("factor", c_float), ("active", c_int32),
+                ("reserved", c_int32)]
 
 
 class PrepareRecord(ctypes.Structure):
@@ -91,6 +102,19 @@ SIGNATURES = [
     ("msr_centralize_bf16", c_int, [c_void_p, c_void_p, c_int64, c_int64, c_float, c_void_p]),
     ("msr_adamw8bit", c_int, [ctypes.POINTER(Adam8Entry), c_int, c_void_p, c_void_p,
                               ctypes.POINTER(Adam8Hparams), c_void_p]),
+    ("msr_grad_norm_workspace_bytes", c_size_t, [c_int]),
+    ("msr_grad_norm", c_int, [c_void_p, c_int, c_int, c_double, c_double, c_void_p, c_void_p, c_void_p, c_size_t,
+                              c_void_p]),
+    ("msr_grad_factor", c_int, [c_void_p, c_int, c_double, c_double, c_void_p]),
+    ("msr_grad_scale", c_int, [c_void_p, c_int, c_void_p, c_void_p]),
+    ("msr_muon_prepare_scaled", c_int, [ctypes.POINTER(PrepareEntry), c_int, c_float, c_float, c_int, c_void_p,
+                                        c_void_p]),
+    ("msr_adamw_sr_scaled", c_int, [ctypes.POINTER(AdamWEntry), c_int, ctypes.POINTER(AdamWHparams), c_void_p,
+                                    c_void_p]),
+    ("msr_muon_prepare_rec_scaled", c_int, [ctypes.POINTER(PrepareEntry), c_int, c_void_p, c_void_p, c_void_p]),
+    ("msr_adamw_sr_rec_scaled", c_int, [ctypes.POINTER(AdamWEntry), c_int, c_void_p, c_void_p, c_void_p]),
+    ("msr_adamw8bit_scaled", c_int, [ctypes.POINTER(Adam8Entry), c_int, c_void_p, c_void_p,
+                                     ctypes.POINTER(Adam8Hparams), c_void_p, c_void_p]),
     ("msr_ns_workspace_bytes", c_size_t, [c_int64, c_int64, c_int64]),
     ("msr_newton_schulz_bf16", c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p,
                                        c_void_p, c_size_t, c_void_p]),

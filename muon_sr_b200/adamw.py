@@ -8,6 +8,7 @@ import random
 import torch
 from torch.optim import Optimizer
 
+from . import clipping
 from . import kernels as K
 from . import staging
 from .seeds import deterministic_seed
@@ -63,23 +64,29 @@ class TritonAdamW(Optimizer):
         eps (float): denominator epsilon (default: 1e-8)
         weight_decay (float): decoupled weight decay (default: 0)
         centralization (float): gradient centralization strength (default: 0)
+
+    ``step(max_norm=, grad_scale=)`` clips the gradients by their global norm as it reads them
+    (see ``clipping``).
     """
+
+    grad_norm = None  # the last step's gradient norm, where it clipped
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0, centralization=0):
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, centralization=centralization)
         super().__init__(params, defaults)
 
     @torch.no_grad()
-    def step(self, closure=None):
+    def step(self, closure=None, max_norm=None, grad_scale=1.0):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        offset = 0
-        for group in self.param_groups:
-            adamw_group_step(self.state, group, offset, deterministic_seed,
-                             centralization=group["centralization"])
-            offset += len(group["params"])
+        with clipping.clipped_step(self, max_norm, grad_scale):
+            offset = 0
+            for group in self.param_groups:
+                adamw_group_step(self.state, group, offset, deterministic_seed,
+                                 centralization=group["centralization"])
+                offset += len(group["params"])
         return loss
 
 

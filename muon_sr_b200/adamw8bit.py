@@ -11,6 +11,7 @@ import math
 import torch
 from torch.optim import Optimizer
 
+from . import clipping
 from . import kernels as K
 from . import staging
 
@@ -83,7 +84,12 @@ class TritonAdamW8bit(Optimizer):
     Default blocks contain 256 elements. Tensors below min_8bit_size=4096 use BF16 moments
     with SR. Set group optim_bits=16 to exclude embeddings/other tensors; for_model() creates
     these groups automatically. CUDA, dense contiguous tensors only.
+
+    ``step(max_norm=, grad_scale=)`` clips the gradients by their global norm as it reads them
+    (see ``clipping``).
     """
+
+    grad_norm = None  # the last step's gradient norm, where it clipped
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0., block_size=256,
                  min_8bit_size=4096, optim_bits=8, shard=None):
@@ -134,11 +140,16 @@ class TritonAdamW8bit(Optimizer):
         return state
 
     @torch.no_grad()
-    def step(self, closure=None):
+    def step(self, closure=None, max_norm=None, grad_scale=1.0):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        with clipping.clipped_step(self, max_norm, grad_scale):
+            self._update()
+        return loss
+
+    def _update(self):
         if self._shard:
             self._shard.bind(self)
         index = 0
@@ -188,7 +199,6 @@ class TritonAdamW8bit(Optimizer):
                     staging.done([e[0] for e in part])
         if self._shard:
             self._shard.sync_params(self)
-        return loss
 
     def load_state_dict(self, state_dict):
         """Checkpoint loading that keeps uint8 codes and fp32 scales (torch's default would cast

@@ -1,0 +1,147 @@
+"""Global gradient norm and clipping on the B200 engine, between the backward pass and the step.
+
+* ``get_total_norm(tensors)`` -- the norm of many gradients taken as one vector.
+* ``clip_grad_norm_(parameters, max_norm)`` -- scales ``.grad`` in place so that this norm is at
+  most ``max_norm``.
+* ``optimizer.step(max_norm=...)``, for every optimizer of this package -- the same clipping
+  without the pass that rewrites the gradients: the update kernels multiply each gradient as
+  they read it. The product is used in fp32, so the result has one bf16 rounding fewer than
+  ``clip_grad_norm_`` followed by ``step()``; ``.grad`` keeps the unclipped values, and
+  ``optimizer.grad_norm`` holds the norm.
+
+The first two take the arguments of their namesakes in ``torch.nn.utils``. Sums are kept in
+double and norms returned in fp32, whatever the gradients' type, on the device: nothing here
+waits for the GPU unless ``error_if_nonfinite`` asks for it.
+"""
+import contextlib
+import math
+
+import torch
+
+from . import kernels as K
+from . import staging
+
+
+def _norm_type(value):
+    value = float(value)
+    if value not in K.NORM_TYPES:
+        raise ValueError(f"norm_type must be 1, 2 or inf, got {value}")
+    return value
+
+
+def _bounds(max_norm, grad_scale):
+    max_norm, grad_scale = float(max_norm), float(grad_scale)
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must be >= 0, got {max_norm}")
+    if not (grad_scale > 0 and math.isfinite(grad_scale)):
+        raise ValueError(f"grad_scale must be positive and finite, got {grad_scale}")
+    return max_norm, grad_scale
+
+
+def _refuse_nonfinite(norm, norm_type):
+    if not math.isfinite(float(norm)):
+        raise RuntimeError(f"The total norm of order {norm_type} for gradients is non-finite, so it cannot be "
+                           "clipped. Pass error_if_nonfinite=False to clip with the non-finite norm anyway.")
+
+
+@torch.no_grad()
+def get_total_norm(tensors, norm_type=2.0, error_if_nonfinite=False, *, per_tensor=False):
+    """The norm of ``tensors`` (bf16, fp16 or fp32 CUDA tensors on one device, mixed at will) as
+    one vector: a 0-dim fp32 tensor on their device, 0 for an empty list.
+
+    ``norm_type`` is 1, 2 or inf. With ``per_tensor`` the result is ``(total, norms)``, the
+    second the fp32 norm of every tensor, from the same pass. ``error_if_nonfinite`` waits for
+    the result and raises ``RuntimeError`` where it is infinite or NaN."""
+    norm_type = _norm_type(norm_type)
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not tensors:
+        total = torch.zeros(())
+        return (total, torch.zeros(0)) if per_tensor else total
+    norm = K.grad_norm(K.GradTable(tensors), norm_type, per_tensor=per_tensor)
+    if error_if_nonfinite:
+        _refuse_nonfinite(norm.norm, norm_type)
+    return (norm.norm, norm.each) if per_tensor else norm.norm
+
+
+def _norm_over_ranks(table, norm_type, grad_scale, max_norm, shard):
+    """The ``GradNorm`` of a table's gradients -- with a sharder, of every rank's together."""
+    norm = K.grad_norm(table, norm_type, grad_scale, max_norm)
+    if shard is not None and shard.world > 1:
+        shard.combine_power(norm.power(norm_type))
+        K.grad_factor(norm, norm_type, grad_scale, max_norm)
+    return norm
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, *, grad_scale=1.0, shard=None):
+    """Multiply the gradients of ``parameters`` in place by
+    ``grad_scale * min(1, max_norm / (norm + 1e-6))``, ``norm`` being the norm of all of them
+    together times ``grad_scale``; returns ``norm`` (0-dim fp32, on their device).
+
+    Arguments:
+        parameters: a parameter or an iterable of them; those without a gradient are passed
+            over, one that is listed twice counts once
+        max_norm (float): the bound; ``math.inf`` clips nothing
+        norm_type (float): 1, 2 or inf
+        error_if_nonfinite (bool): wait for the norm and raise ``RuntimeError``, the gradients
+            untouched, where it is infinite or NaN. Otherwise a NaN norm makes every gradient
+            NaN and an infinite one makes them 0 (NaN where they were infinite)
+        grad_scale (float): multiplies every gradient in any case, e.g. 1 / micro-batches
+        shard: the ``Sharder`` whose ``reduce_grads`` has brought each gradient to its owner.
+            Collective: the norm is over all ranks' gradients, each rank scales those it owns
+
+    Gradients whose norm is within the bound are not written (``grad_scale`` 1). Two parameters
+    whose gradients share memory are refused."""
+    norm_type = _norm_type(norm_type)
+    max_norm, grad_scale = _bounds(max_norm, grad_scale)
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(dict.fromkeys(parameters))
+    params = [p for p in parameters if p.grad is not None]
+    device = _device(params)
+    if shard is not None:
+        params = shard.owned(params)
+    if device is None:
+        if shard is None:
+            return torch.zeros(())
+        device = torch.device("cuda", torch.cuda.current_device())
+    grads = [p.grad for p in params]
+    for g in grads:
+        if g.layout is torch.strided and not g.is_contiguous() and \
+                any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
+            raise ValueError("gradients must not be expanded tensors: their elements share memory")
+    table = K.GradTable(grads, device)
+    norm = _norm_over_ranks(table, norm_type, grad_scale, max_norm, shard)
+    if error_if_nonfinite:
+        _refuse_nonfinite(norm.norm, norm_type)
+    K.grad_scale_(table, norm)
+    return norm.norm
+
+
+def _device(params):
+    return params[0].grad.device if params else None
+
+
+def clipped_step(optimizer, max_norm, grad_scale):
+    """The context in which an optimizer's ``step`` issues its launches: with ``max_norm``, the
+    norm of all its gradients is launched here and the step's kernels read every gradient times
+    the factor; ``optimizer.grad_norm`` is that norm, or None without ``max_norm``."""
+    optimizer.grad_norm = None
+    if max_norm is None:
+        if grad_scale != 1.0:
+            raise ValueError("grad_scale needs max_norm (math.inf clips nothing)")
+        return contextlib.nullcontext()
+    max_norm, grad_scale = _bounds(max_norm, grad_scale)
+    params = list(dict.fromkeys(p for g in optimizer.param_groups for p in g["params"] if p.grad is not None))
+    device = _device(params)
+    shard = getattr(optimizer, "_shard", None)
+    if shard is not None:
+        shard._ensure(optimizer)
+        params = shard.owned(params)
+    if device is None:
+        if shard is None:
+            return contextlib.nullcontext()
+        device = torch.device("cuda", torch.cuda.current_device())
+    staging.need(params)
+    table = K.GradTable([p.grad for p in params], device)
+    norm = _norm_over_ranks(table, 2.0, grad_scale, max_norm, shard)
+    optimizer.grad_norm = norm.norm
+    return K.gradient_factor(norm.factor)

@@ -33,6 +33,7 @@ struct Adam8Args {
   const float* qmap1;
   const float* qmap2;
   int any_mc;  // some entry stores its weights through a multicast address
+  const float* gscale;  // msr_adamw8bit_scaled: what the gradients are multiplied by
 };
 
 __device__ __forceinline__ float fadd(float a, float b) { return __fadd_rn(a, b); }
@@ -129,7 +130,7 @@ __device__ __forceinline__ float group_max(float v, float* red) {
 constexpr size_t smem_for(bool tables) { return 2 * 256 * 4 + (tables ? MSR_QT_BYTES : 0); }
 
 // EPT elements per thread, BS elements per quantisation block.
-template <int BS, bool TABLES, int NOISE>
+template <int BS, bool TABLES, int NOISE, bool SCALED>
 __global__ __launch_bounds__(Q_THREADS, 4) void adamw8bit_kernel(const __grid_constant__ Adam8Args a) {
   constexpr bool FAST = NOISE == NOISE_FAST;
   constexpr int EPT = BS > 2048 ? 16 : 8;
@@ -156,6 +157,7 @@ __global__ __launch_bounds__(Q_THREADS, 4) void adamw8bit_kernel(const __grid_co
   const float* t_pos2 = t_pos1 + 512;
   __syncthreads();
   const msr_adamw8bit_hparams hp = a.hp;
+  const float gs = SCALED ? *a.gscale : 1.f;
   const int64_t total = a.prefix[a.count];
   int ei = blockIdx.x < total ? find_entry<Q_MAXE>(a.prefix, a.count, blockIdx.x) : 0;
   for (int64_t tile = blockIdx.x; tile < total; tile += gridDim.x) {
@@ -249,7 +251,8 @@ __global__ __launch_bounds__(Q_THREADS, 4) void adamw8bit_kernel(const __grid_co
     float mmax = 0.f, vmax = 0.f;
 #pragma unroll
     for (int j = 0; j < EPT; ++j) {
-      const float g = bf16_bits_to_f32(gb[j]);
+      float g = bf16_bits_to_f32(gb[j]);
+      if (SCALED) g = fmul(g, gs);  // not rounded to bf16 in between
       const bool fin = finite_f(g);
       m[j] = fin ? fadd(fmul(hp.beta1, m[j]), fmul(hp.one_minus_beta1, g)) : 0.f;
       v[j] = fin ? fadd(fmul(hp.beta2, v[j]), fmul(fmul(hp.one_minus_beta2, g), g)) : 0.f;
@@ -369,23 +372,27 @@ __global__ __launch_bounds__(Q_THREADS, 4) void adamw8bit_kernel(const __grid_co
   if (a.any_mc) __threadfence_system();
 }
 
-template <int BS, bool TABLES, int NOISE>
+template <int BS, bool TABLES, int NOISE, bool SCALED>
 int launch_variant(const Adam8Args& a, int64_t tiles, cudaStream_t s) {
   const int64_t cap = static_cast<int64_t>(sm_count()) * Q_BLOCKS_PER_SM;
   const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles, cap)));
   constexpr size_t smem = smem_for(TABLES);
   if (smem > 48 * 1024) {
-    if (int st = set_smem_attr(reinterpret_cast<const void*>(adamw8bit_kernel<BS, TABLES, NOISE>), smem,
+    if (int st = set_smem_attr(reinterpret_cast<const void*>(adamw8bit_kernel<BS, TABLES, NOISE, SCALED>), smem,
                                "adamw8bit_kernel"))
       return st;
   }
-  adamw8bit_kernel<BS, TABLES, NOISE><<<grid, Q_THREADS, smem, s>>>(a);
+  adamw8bit_kernel<BS, TABLES, NOISE, SCALED><<<grid, Q_THREADS, smem, s>>>(a);
   return check_launch("adamw8bit_kernel");
 }
 
 template <int BS, int NOISE>
 int launch_noise(const Adam8Args& a, int64_t tiles, cudaStream_t s) {
-  return a.hp.qtables ? launch_variant<BS, true, NOISE>(a, tiles, s) : launch_variant<BS, false, NOISE>(a, tiles, s);
+  if (a.gscale)
+    return a.hp.qtables ? launch_variant<BS, true, NOISE, true>(a, tiles, s)
+                        : launch_variant<BS, false, NOISE, true>(a, tiles, s);
+  return a.hp.qtables ? launch_variant<BS, true, NOISE, false>(a, tiles, s)
+                      : launch_variant<BS, false, NOISE, false>(a, tiles, s);
 }
 
 template <int BS>
@@ -395,13 +402,8 @@ int launch_bs(const Adam8Args& a, int64_t tiles, cudaStream_t s) {
 
 inline bool al(const void* p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
-}  // namespace
-}  // namespace msr
-
-using namespace msr;
-
-extern "C" int msr_adamw8bit(const msr_adamw8bit_entry* entries, int count, const float* qmap1, const float* qmap2,
-                             const msr_adamw8bit_hparams* hp, msr_stream_t stream) {
+int adamw8bit_launch(const msr_adamw8bit_entry* entries, int count, const float* qmap1, const float* qmap2,
+                     const msr_adamw8bit_hparams* hp, const float* gscale, msr_stream_t stream) {
   if (count < 0 || (count > 0 && (entries == nullptr || hp == nullptr)))
     return fail(MSR_ERR_INVALID, "msr_adamw8bit: bad entry list or hparams");
   const int bs = hp->block_size;
@@ -415,6 +417,7 @@ extern "C" int msr_adamw8bit(const msr_adamw8bit_entry* entries, int count, cons
     a.hp = *hp;
     a.qmap1 = qmap1;
     a.qmap2 = qmap2;
+    a.gscale = gscale;
     int64_t tiles = 0;
     bool any_quant = false;
     int i = next;
@@ -459,3 +462,24 @@ extern "C" int msr_adamw8bit(const msr_adamw8bit_entry* entries, int count, cons
   }
   return MSR_OK;
 }
+
+}  // namespace
+}  // namespace msr
+
+using namespace msr;
+
+extern "C" {
+
+int msr_adamw8bit(const msr_adamw8bit_entry* entries, int count, const float* qmap1, const float* qmap2,
+                  const msr_adamw8bit_hparams* hp, msr_stream_t stream) {
+  return adamw8bit_launch(entries, count, qmap1, qmap2, hp, nullptr, stream);
+}
+
+int msr_adamw8bit_scaled(const msr_adamw8bit_entry* entries, int count, const float* qmap1, const float* qmap2,
+                         const msr_adamw8bit_hparams* hp, const float* grad_factor, msr_stream_t stream) {
+  if (!grad_factor || !al(grad_factor, 4))
+    return fail(MSR_ERR_INVALID, "msr_adamw8bit_scaled: bad grad_factor pointer");
+  return adamw8bit_launch(entries, count, qmap1, qmap2, hp, grad_factor, stream);
+}
+
+}  // extern "C"

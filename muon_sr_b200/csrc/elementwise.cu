@@ -10,7 +10,8 @@
 // results are bit-identical to the reference kernels' fp32 evaluation. Every kernel is
 // instantiated per noise mode (msr_set_sr_noise), and prepare / apply / AdamW once more
 // (REC) for the replayable launches that read their scalars and entries from a device
-// record (msr_*_rec, used inside captured CUDA graphs).
+// record (msr_*_rec, used inside captured CUDA graphs). Prepare and AdamW come once more
+// (SCALED) with the gradient multiplied by a device scalar as it is read (msr_*_scaled).
 #include "common.cuh"
 #include "host_common.h"
 
@@ -134,6 +135,7 @@ struct PrepareArgs {
   // record; src[i] is the record's index of entry i.
   const msr_prepare_record* rec;
   int32_t src[MAXE];
+  const float* gscale;  // msr_muon_prepare_scaled: what the gradients are multiplied by
 };
 
 // Launch scalars and entry i of a launch, from the parameters or (REC) the device record.
@@ -147,12 +149,20 @@ __device__ __forceinline__ float beta_of(const PrepareArgs& a) { return REC ? a.
 template <bool REC>
 __device__ __forceinline__ float omb_of(const PrepareArgs& a) { return REC ? a.rec->one_minus_beta : a.omb; }
 
+// A gradient as the update uses it. The scaled product stays in fp32: one rounding fewer than
+// scaling the bf16 gradient in memory first.
+template <bool SCALED>
+__device__ __forceinline__ float grad_value(uint16_t bits, float gs) {
+  const float g = bf16_bits_to_f32(bits);
+  return SCALED ? fmul(g, gs) : g;
+}
+
 // `rnd()` yields the element's noise word; it is called after the math, where the noise is
 // consumed, which keeps the register allocation of the Philox chain as short as possible.
-template <int NOISE, class Rnd>
-__device__ __forceinline__ void prepare_one(uint16_t g_bits, uint16_t b_bits, float beta, float omb, bool nesterov,
-                                            Rnd rnd, uint16_t& buf_out, uint16_t& upd_out) {
-  const float g = bf16_bits_to_f32(g_bits);
+template <int NOISE, bool SCALED, class Rnd>
+__device__ __forceinline__ void prepare_one(uint16_t g_bits, float gs, uint16_t b_bits, float beta, float omb,
+                                            bool nesterov, Rnd rnd, uint16_t& buf_out, uint16_t& upd_out) {
+  const float g = grad_value<SCALED>(g_bits, gs);
   const float buf = bf16_bits_to_f32(b_bits);
   const float nb = fadd(buf, fmul(omb, fsub(g, buf)));
   const float upd = nesterov ? fadd(g, fmul(beta, fsub(nb, g))) : nb;
@@ -160,9 +170,10 @@ __device__ __forceinline__ void prepare_one(uint16_t g_bits, uint16_t b_bits, fl
   upd_out = rne_bf16_bits(upd);
 }
 
-template <int NOISE, bool REC>
+template <int NOISE, bool REC, bool SCALED>
 __global__ __launch_bounds__(EW_THREADS, 4) void muon_prepare_kernel(const __grid_constant__ PrepareArgs a) {
   constexpr bool FAST = NOISE == NOISE_FAST;
+  const float gs = SCALED ? *a.gscale : 1.f;
   const int64_t total = a.prefix[a.count];
   const bool nesterov = (REC ? a.rec->nesterov : a.nesterov) != 0;
   for (int64_t chunk = blockIdx.x; chunk < total; chunk += gridDim.x) {
@@ -194,7 +205,7 @@ __global__ __launch_bounds__(EW_THREADS, 4) void muon_prepare_kernel(const __gri
           if (FAST) nz.eight(cb + static_cast<uint64_t>(idx), r);
 #pragma unroll
           for (int j = 0; j < EW_VEC; ++j)
-            prepare_one<NOISE>(vg[it].v[j], vb[it].v[j], beta_of<REC>(a), omb_of<REC>(a), nesterov,
+            prepare_one<NOISE, SCALED>(vg[it].v[j], gs, vb[it].v[j], beta_of<REC>(a), omb_of<REC>(a), nesterov,
                                [&] { return FAST ? r[j] : nz.at(cb + static_cast<uint64_t>(idx + j)); }, ob.v[j],
                                ou.v[j]);
           st_u16x8(mb + idx, ob);
@@ -202,7 +213,8 @@ __global__ __launch_bounds__(EW_THREADS, 4) void muon_prepare_kernel(const __gri
         } else {
           for (int64_t i = idx; i < n; ++i) {
             uint16_t ob, ou;
-            prepare_one<NOISE>(g[i], mb[i], beta_of<REC>(a), omb_of<REC>(a), nesterov, [&] { return nz.at(cb + static_cast<uint64_t>(i)); }, ob, ou);
+            prepare_one<NOISE, SCALED>(g[i], gs, mb[i], beta_of<REC>(a), omb_of<REC>(a), nesterov,
+                                       [&] { return nz.at(cb + static_cast<uint64_t>(i)); }, ob, ou);
             mb[i] = ob;
             up[i] = ou;
           }
@@ -213,7 +225,8 @@ __global__ __launch_bounds__(EW_THREADS, 4) void muon_prepare_kernel(const __gri
         const int64_t i = base + it * EW_THREADS + threadIdx.x;
         if (i < n) {
           uint16_t ob, ou;
-          prepare_one<NOISE>(g[i], mb[i], beta_of<REC>(a), omb_of<REC>(a), nesterov, [&] { return nz.at(cb + static_cast<uint64_t>(i)); }, ob, ou);
+          prepare_one<NOISE, SCALED>(g[i], gs, mb[i], beta_of<REC>(a), omb_of<REC>(a), nesterov,
+                                       [&] { return nz.at(cb + static_cast<uint64_t>(i)); }, ob, ou);
           mb[i] = ob;
           up[i] = ou;
         }
@@ -344,6 +357,7 @@ struct AdamWArgs {
   const msr_adamw_record* rec;  // msr_adamw_sr_rec (see PrepareArgs)
   int32_t src[MAXE];
   int any_mc;  // some entry stores its weights through a multicast address
+  const float* gscale;  // msr_adamw_sr_scaled: what the gradients are multiplied by
 };
 
 template <bool REC>
@@ -357,10 +371,11 @@ __device__ __forceinline__ const msr_adamw_hparams& hp_of(const AdamWArgs& a) {
   else return a.hp;
 }
 
-template <int NOISE, class Rnd>
-__device__ __forceinline__ void adamw_one(uint16_t& p_bits, uint16_t g_bits, uint16_t& m_bits, uint16_t& v_bits,
-                                          const msr_adamw_hparams& hp, float step_size, float bc2s, Rnd rnd) {
-  const float g = bf16_bits_to_f32(g_bits);
+template <int NOISE, bool SCALED, class Rnd>
+__device__ __forceinline__ void adamw_one(uint16_t& p_bits, uint16_t g_bits, float gs, uint16_t& m_bits,
+                                          uint16_t& v_bits, const msr_adamw_hparams& hp, float step_size, float bc2s,
+                                          Rnd rnd) {
+  const float g = grad_value<SCALED>(g_bits, gs);
   float m = bf16_bits_to_f32(m_bits);
   float v = bf16_bits_to_f32(v_bits);
   float p = bf16_bits_to_f32(p_bits);
@@ -377,10 +392,10 @@ __device__ __forceinline__ void adamw_one(uint16_t& p_bits, uint16_t g_bits, uin
 // Elements lo .. hi - 1 of one AdamW entry, one thread: plain stores, or (multicast weights)
 // the weights in 4-byte pairs from an even index (a pair past the last element writes 0 into
 // the padding that follows the parameter's slot); the moments are always local.
-template <int NOISE, bool REC>
-__device__ __forceinline__ void adamw_tail(const AdamWArgs& a, const msr_adamw_entry& E, const SrNoise<NOISE>& nm,
-                                           const SrNoise<NOISE>& nv, const SrNoise<NOISE>& np_, int64_t lo,
-                                           int64_t hi) {
+template <int NOISE, bool REC, bool SCALED>
+__device__ __forceinline__ void adamw_tail(const AdamWArgs& a, const msr_adamw_entry& E, float gs,
+                                           const SrNoise<NOISE>& nm, const SrNoise<NOISE>& nv,
+                                           const SrNoise<NOISE>& np_, int64_t lo, int64_t hi) {
   uint16_t* p = static_cast<uint16_t*>(E.param);
   uint16_t* pm = static_cast<uint16_t*>(E.param_mc);
   const uint16_t* g = static_cast<const uint16_t*>(E.grad);
@@ -389,7 +404,7 @@ __device__ __forceinline__ void adamw_tail(const AdamWArgs& a, const msr_adamw_e
   auto one = [&](int64_t i) {
     uint16_t pb = p[i], mb = m[i], vb = v[i];
     const uint64_t c = static_cast<uint64_t>(i);
-    adamw_one<NOISE>(pb, g[i], mb, vb, hp_of<REC>(a), E.step_size, E.bc2_sqrt,
+    adamw_one<NOISE, SCALED>(pb, g[i], gs, mb, vb, hp_of<REC>(a), E.step_size, E.bc2_sqrt,
                      [&](int w) { return w == 0 ? nm.at(c) : w == 1 ? nv.at(c) : np_.at(c); });
     m[i] = mb;
     v[i] = vb;
@@ -406,9 +421,10 @@ __device__ __forceinline__ void adamw_tail(const AdamWArgs& a, const msr_adamw_e
 }
 
 // ITERS vectors of 8 elements per thread and chunk; MINB CTAs per SM for the register budget.
-template <int ITERS, int MINB, int NOISE, bool REC>
+template <int ITERS, int MINB, int NOISE, bool REC, bool SCALED>
 __global__ __launch_bounds__(EW_THREADS, MINB) void adamw_kernel(const __grid_constant__ AdamWArgs a) {
   constexpr bool FAST = NOISE == NOISE_FAST;
+  const float gs = SCALED ? *a.gscale : 1.f;
   constexpr int64_t CHUNK = EW_THREADS * EW_VEC * ITERS;
   const int64_t total = a.prefix[a.count];
   for (int64_t chunk = blockIdx.x; chunk < total; chunk += gridDim.x) {
@@ -448,7 +464,7 @@ __global__ __launch_bounds__(EW_THREADS, MINB) void adamw_kernel(const __grid_co
 #pragma unroll
           for (int j = 0; j < EW_VEC; ++j) {
             const uint64_t c = static_cast<uint64_t>(idx + j);
-            adamw_one<NOISE>(vp[it].v[j], vg[it].v[j], vm[it].v[j], vv[it].v[j], hp_of<REC>(a), ss, bc2s, [&](int w) {
+            adamw_one<NOISE, SCALED>(vp[it].v[j], vg[it].v[j], gs, vm[it].v[j], vv[it].v[j], hp_of<REC>(a), ss, bc2s, [&](int w) {
               return w == 0 ? (FAST ? rm[j] : nm.at(c)) : w == 1 ? (FAST ? rv[j] : nv.at(c)) : (FAST ? rp[j] : np_.at(c));
             });
           }
@@ -459,18 +475,18 @@ __global__ __launch_bounds__(EW_THREADS, MINB) void adamw_kernel(const __grid_co
           st_u16x8(m + idx, vm[it]);
           st_u16x8(v + idx, vv[it]);
         } else {
-          adamw_tail<NOISE, REC>(a, E, nm, nv, np_, idx, n);
+          adamw_tail<NOISE, REC, SCALED>(a, E, gs, nm, nv, np_, idx, n);
         }
       }
     } else if (pm) {  // an unaligned entry with multicast weights: 4-byte pairs, thread-contiguous
       const int64_t lo = base + static_cast<int64_t>(threadIdx.x) * (ITERS * EW_VEC);
-      adamw_tail<NOISE, REC>(a, E, nm, nv, np_, lo, lo + ITERS * EW_VEC < n ? lo + ITERS * EW_VEC : n);
+      adamw_tail<NOISE, REC, SCALED>(a, E, gs, nm, nv, np_, lo, lo + ITERS * EW_VEC < n ? lo + ITERS * EW_VEC : n);
     } else {
       for (int it = 0; it < ITERS * EW_VEC; ++it) {
         const int64_t i = base + it * EW_THREADS + threadIdx.x;
         if (i < n) {
           uint16_t pb = p[i], mb = m[i], vb = v[i];
-          adamw_one<NOISE>(pb, g[i], mb, vb, hp_of<REC>(a), ss, bc2s, [&](int w) {
+          adamw_one<NOISE, SCALED>(pb, g[i], gs, mb, vb, hp_of<REC>(a), ss, bc2s, [&](int w) {
               const uint64_t c = static_cast<uint64_t>(i);
               return w == 0 ? nm.at(c) : w == 1 ? nv.at(c) : np_.at(c);
             });
@@ -542,11 +558,19 @@ inline int grid_for(int64_t chunks) {
 
 inline bool record_ok(const void* rec) { return rec != nullptr && (reinterpret_cast<uintptr_t>(rec) & 15u) == 0; }
 
+inline bool factor_ok(const float* f) { return f != nullptr && (reinterpret_cast<uintptr_t>(f) & 3u) == 0; }
+
 // The multi-tensor launchers: entries are packed MAXE at a time (empty ones skipped, each
 // group resuming at the first entry the previous one did not take); with a record, the
 // kernels take scalars and entries from it (src[] maps packed to record indices).
+template <bool REC, bool SCALED>
+auto* prepare_kernel() {
+  return pick_noise(muon_prepare_kernel<NOISE_REF, REC, SCALED>, muon_prepare_kernel<NOISE_FAST, REC, SCALED>,
+                    muon_prepare_kernel<NOISE_NONE, REC, SCALED>);
+}
+
 int prepare_launch(const msr_prepare_entry* entries, int count, float beta, float one_minus_beta, int nesterov,
-                   const msr_prepare_record* rec, msr_stream_t stream) {
+                   const msr_prepare_record* rec, const float* gscale, msr_stream_t stream) {
   if (count < 0 || (count > 0 && entries == nullptr)) return fail(MSR_ERR_INVALID, "msr_muon_prepare: bad entry list");
   int next = 0;
   while (next < count) {
@@ -555,6 +579,7 @@ int prepare_launch(const msr_prepare_entry* entries, int count, float beta, floa
     a.omb = one_minus_beta;
     a.nesterov = nesterov;
     a.rec = rec;
+    a.gscale = gscale;
     int64_t chunks = 0;
     int i = next;
     for (; i < count && a.count < MAXE; ++i) {
@@ -572,10 +597,8 @@ int prepare_launch(const msr_prepare_entry* entries, int count, float beta, floa
     next = i;
     a.prefix[a.count] = chunks;
     if (a.count == 0) continue;
-    auto* kern = rec ? pick_noise(muon_prepare_kernel<NOISE_REF, true>, muon_prepare_kernel<NOISE_FAST, true>,
-                                  muon_prepare_kernel<NOISE_NONE, true>)
-                     : pick_noise(muon_prepare_kernel<NOISE_REF, false>, muon_prepare_kernel<NOISE_FAST, false>,
-                                  muon_prepare_kernel<NOISE_NONE, false>);
+    auto* kern = rec ? (gscale ? prepare_kernel<true, true>() : prepare_kernel<true, false>())
+                     : (gscale ? prepare_kernel<false, true>() : prepare_kernel<false, false>());
     kern<<<grid_for(chunks), EW_THREADS, 0, to_stream(stream)>>>(a);
     int st = check_launch("muon_prepare_kernel");
     if (st) return st;
@@ -623,8 +646,15 @@ int apply_launch(const msr_apply_entry* entries, int count, float lr, float deca
   return MSR_OK;
 }
 
+template <bool REC, bool SCALED>
+auto* adamw_kernel_for() {
+  return pick_noise(adamw_kernel<ADAMW_ITERS, ADAMW_MINB, NOISE_REF, REC, SCALED>,
+                    adamw_kernel<ADAMW_ITERS, ADAMW_MINB, NOISE_FAST, REC, SCALED>,
+                    adamw_kernel<ADAMW_ITERS, ADAMW_MINB, NOISE_NONE, REC, SCALED>);
+}
+
 int adamw_launch(const msr_adamw_entry* entries, int count, const msr_adamw_hparams* hp, const msr_adamw_record* rec,
-                 msr_stream_t stream) {
+                 const float* gscale, msr_stream_t stream) {
   if (count < 0 || (count > 0 && entries == nullptr))
     return fail(MSR_ERR_INVALID, "msr_adamw_sr: bad entry list or hparams");
   int next = 0;
@@ -632,6 +662,7 @@ int adamw_launch(const msr_adamw_entry* entries, int count, const msr_adamw_hpar
     AdamWArgs a{};
     if (hp) a.hp = *hp;
     a.rec = rec;
+    a.gscale = gscale;
     int64_t chunks = 0;
     int i = next;
     for (; i < count && a.count < MAXE; ++i) {
@@ -653,12 +684,8 @@ int adamw_launch(const msr_adamw_entry* entries, int count, const msr_adamw_hpar
     next = i;
     a.prefix[a.count] = chunks;
     if (a.count == 0) continue;
-    auto* kern = rec ? pick_noise(adamw_kernel<ADAMW_ITERS, ADAMW_MINB, NOISE_REF, true>,
-                                  adamw_kernel<ADAMW_ITERS, ADAMW_MINB, NOISE_FAST, true>,
-                                  adamw_kernel<ADAMW_ITERS, ADAMW_MINB, NOISE_NONE, true>)
-                     : pick_noise(adamw_kernel<ADAMW_ITERS, ADAMW_MINB, NOISE_REF, false>,
-                                  adamw_kernel<ADAMW_ITERS, ADAMW_MINB, NOISE_FAST, false>,
-                                  adamw_kernel<ADAMW_ITERS, ADAMW_MINB, NOISE_NONE, false>);
+    auto* kern = rec ? (gscale ? adamw_kernel_for<true, true>() : adamw_kernel_for<true, false>())
+                     : (gscale ? adamw_kernel_for<false, true>() : adamw_kernel_for<false, false>());
     // one wave of resident CTAs (ADAMW_MINB per SM), each walking its chunks
     const int64_t cap = static_cast<int64_t>(sm_count()) * ADAMW_MINB;
     const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(chunks, cap)));
@@ -724,12 +751,13 @@ int msr_grad_accum_bf16(void* acc, const void* grad, int64_t n, uint64_t key, in
 
 int msr_muon_prepare(const msr_prepare_entry* entries, int count, float beta, float one_minus_beta, int nesterov,
                      msr_stream_t stream) {
-  return msr::prepare_launch(entries, count, beta, one_minus_beta, nesterov, nullptr, stream);
+  return msr::prepare_launch(entries, count, beta, one_minus_beta, nesterov, nullptr, nullptr, stream);
 }
 
 int msr_muon_prepare_rec(const msr_prepare_entry* entries, int count, const void* record, msr_stream_t stream) {
   if (!msr::record_ok(record)) return fail(MSR_ERR_INVALID, "msr_muon_prepare_rec: record must be 16-byte aligned");
-  return msr::prepare_launch(entries, count, 0.f, 0.f, 0, static_cast<const msr_prepare_record*>(record), stream);
+  return msr::prepare_launch(entries, count, 0.f, 0.f, 0, static_cast<const msr_prepare_record*>(record), nullptr,
+                             stream);
 }
 
 int msr_muon_apply(const msr_apply_entry* entries, int count, float lr, float decay, msr_stream_t stream) {
@@ -743,12 +771,41 @@ int msr_muon_apply_rec(const msr_apply_entry* entries, int count, const void* re
 
 int msr_adamw_sr(const msr_adamw_entry* entries, int count, const msr_adamw_hparams* hp, msr_stream_t stream) {
   if (count > 0 && hp == nullptr) return fail(MSR_ERR_INVALID, "msr_adamw_sr: bad entry list or hparams");
-  return msr::adamw_launch(entries, count, hp, nullptr, stream);
+  return msr::adamw_launch(entries, count, hp, nullptr, nullptr, stream);
 }
 
 int msr_adamw_sr_rec(const msr_adamw_entry* entries, int count, const void* record, msr_stream_t stream) {
   if (!msr::record_ok(record)) return fail(MSR_ERR_INVALID, "msr_adamw_sr_rec: record must be 16-byte aligned");
-  return msr::adamw_launch(entries, count, nullptr, static_cast<const msr_adamw_record*>(record), stream);
+  return msr::adamw_launch(entries, count, nullptr, static_cast<const msr_adamw_record*>(record), nullptr, stream);
+}
+
+int msr_muon_prepare_scaled(const msr_prepare_entry* entries, int count, float beta, float one_minus_beta, int nesterov,
+                            const float* grad_factor, msr_stream_t stream) {
+  if (!msr::factor_ok(grad_factor)) return fail(MSR_ERR_INVALID, "msr_muon_prepare_scaled: bad grad_factor pointer");
+  return msr::prepare_launch(entries, count, beta, one_minus_beta, nesterov, nullptr, grad_factor, stream);
+}
+
+int msr_muon_prepare_rec_scaled(const msr_prepare_entry* entries, int count, const void* record,
+                                const float* grad_factor, msr_stream_t stream) {
+  if (!msr::record_ok(record))
+    return fail(MSR_ERR_INVALID, "msr_muon_prepare_rec_scaled: record must be 16-byte aligned");
+  if (!msr::factor_ok(grad_factor)) return fail(MSR_ERR_INVALID, "msr_muon_prepare_rec_scaled: bad grad_factor pointer");
+  return msr::prepare_launch(entries, count, 0.f, 0.f, 0, static_cast<const msr_prepare_record*>(record), grad_factor,
+                             stream);
+}
+
+int msr_adamw_sr_scaled(const msr_adamw_entry* entries, int count, const msr_adamw_hparams* hp,
+                        const float* grad_factor, msr_stream_t stream) {
+  if (count > 0 && hp == nullptr) return fail(MSR_ERR_INVALID, "msr_adamw_sr_scaled: bad entry list or hparams");
+  if (!msr::factor_ok(grad_factor)) return fail(MSR_ERR_INVALID, "msr_adamw_sr_scaled: bad grad_factor pointer");
+  return msr::adamw_launch(entries, count, hp, nullptr, grad_factor, stream);
+}
+
+int msr_adamw_sr_rec_scaled(const msr_adamw_entry* entries, int count, const void* record, const float* grad_factor,
+                            msr_stream_t stream) {
+  if (!msr::record_ok(record)) return fail(MSR_ERR_INVALID, "msr_adamw_sr_rec_scaled: record must be 16-byte aligned");
+  if (!msr::factor_ok(grad_factor)) return fail(MSR_ERR_INVALID, "msr_adamw_sr_rec_scaled: bad grad_factor pointer");
+  return msr::adamw_launch(entries, count, nullptr, static_cast<const msr_adamw_record*>(record), grad_factor, stream);
 }
 
 }  // extern "C"

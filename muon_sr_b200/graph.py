@@ -42,6 +42,9 @@ _SCALAR_FIELDS = {
     "msr_muon_apply_rec": ("key", "scale"),
     "msr_adamw_sr_rec": ("key_m", "key_v", "key_p", "step_size", "bc2_sqrt"),
 }
+# The launches that read their gradients times a device scalar have the same records.
+for _fn in ("msr_muon_prepare_rec", "msr_adamw_sr_rec"):
+    _SCALAR_FIELDS[_fn + "_scaled"] = _SCALAR_FIELDS[_fn]
 
 _CHANGED = ("the optimizer step no longer matches its captured graph (parameters with gradients, "
             "gradient tensors, shapes, baked-in constants or the launch sequence changed); build a new StepGraph")
@@ -90,7 +93,9 @@ class _Recorder:
             self.constants.append((name, value))
         self.seen += 1
 
-    def launch(self, fn, header, entries, device):
+    def launch(self, fn, header, entries, device, factor=None):
+        if factor is not None:
+            fn += "_scaled"
         if self.mode == "refresh":
             self._refresh(fn, header, entries)
             return
@@ -101,8 +106,9 @@ class _Recorder:
             if self.size > self.host.numel():
                 raise RuntimeError(_CHANGED)
             self._write(launch)
+            scalar = () if factor is None else (factor.data_ptr(),)
             status = getattr(_lib.load(), fn)(entries, len(entries), ctypes.c_void_p(self.dev.data_ptr() + offset),
-                                              K.stream_handle(device))
+                                              *scalar, K.stream_handle(device))
             _lib.check(status, fn)
         self.plan.append(launch)
 
@@ -134,11 +140,11 @@ def _snapshot(opt):
     batched groups' global step and torch's CPU generator (seeds of the MuonSR classes)."""
     state = {p: {k: v for k, v in st.items() if not torch.is_tensor(v)} for p, st in opt.state.items()}
     clock = getattr(opt, "_clock", None)
-    return state, (clock.value if clock is not None else None), torch.get_rng_state()
+    return state, (clock.value if clock is not None else None), torch.get_rng_state(), opt.grad_norm
 
 
 def _restore(opt, snap):
-    state, clock, rng = snap
+    state, clock, rng, opt.grad_norm = snap
     for p in list(opt.state.keys()):
         saved = state.get(p)
         if saved is None:
@@ -154,7 +160,7 @@ def _restore(opt, snap):
 
 
 class _Slot:
-    __slots__ = ("graph", "host", "dev", "plan", "constants", "done", "held")
+    __slots__ = ("graph", "host", "dev", "plan", "constants", "done", "held", "grad_norm")
 
 
 class StepGraph:
@@ -164,9 +170,12 @@ class StepGraph:
         optimizer: a TritonMuonSR, TritonMuonSRWithAuxAdam, MuonSR, MuonSRWithAuxAdam or
             TritonAdamW that has run one eager step with the gradients the replays will use
         copies: graphs replayed alternately (2 lets the host refresh one while the other runs)
+        max_norm, grad_scale: those of the captured ``optimizer.step(max_norm=, grad_scale=)``,
+            fixed for the life of the graph. ``optimizer.grad_norm`` after a replay is that
+            replay's norm, to be read before ``copies`` further steps have overwritten it
     """
 
-    def __init__(self, optimizer, copies: int = 2):
+    def __init__(self, optimizer, copies: int = 2, max_norm=None, grad_scale: float = 1.0):
         from .adamw import TritonAdamW
         from .muon import _MuonBase
         if not isinstance(optimizer, (_MuonBase, TritonAdamW)):
@@ -176,6 +185,7 @@ class StepGraph:
         if copies < 1:
             raise ValueError("copies must be >= 1")
         self.optimizer = optimizer
+        self._clip = {} if max_norm is None and grad_scale == 1.0 else dict(max_norm=max_norm, grad_scale=grad_scale)
         self._params = [p for g in optimizer.param_groups for p in g["params"]]
         with_grad = [p for p in self._params if p.grad is not None]
         if not with_grad:
@@ -200,7 +210,8 @@ class StepGraph:
             try:
                 with K.recorder(rec), torch.cuda.graph(s.graph, pool=pool):
                     s.dev.copy_(s.host, non_blocking=True)
-                    optimizer.step()
+                    optimizer.step(**self._clip)
+                s.grad_norm = optimizer.grad_norm
             finally:
                 _restore(optimizer, snap)
             if [x.numels for x in rec.plan] != [x.numels for x in sizing.plan] or rec.constants != sizing.constants:
@@ -233,7 +244,7 @@ class StepGraph:
         snap = _snapshot(self.optimizer)
         try:
             with K.recorder(rec):
-                self.optimizer.step()
+                self.optimizer.step(**self._clip)
         finally:
             _restore(self.optimizer, snap)
         return rec
@@ -249,7 +260,7 @@ class StepGraph:
         ok = False
         try:
             with K.recorder(rec):
-                self.optimizer.step()
+                self.optimizer.step(**self._clip)
             # the pass itself may have moved state (momentum stacks rebuilt after a load)
             ok = rec.complete() and self._storage_ptrs() == self._storage
         finally:
@@ -258,5 +269,6 @@ class StepGraph:
         if not ok:
             raise RuntimeError(_CHANGED)
         s.graph.replay()
+        self.optimizer.grad_norm = s.grad_norm
         s.done.record()
         self._next = (self._next + 1) % len(self._slots)

@@ -5,6 +5,7 @@ Scalars that the reference evaluates from Python floats (``1 - beta``, ``1 - lr 
 ``lr / bias_correction`` ...) are computed here in double and rounded to fp32 once, as the
 reference's kernels see them.
 """
+import array
 import contextlib
 import ctypes
 import math
@@ -59,6 +60,23 @@ def _recorder():
 def _issuing():
     rec = _recorder()
     return rec is None or rec.launches
+
+
+# ``gradient_factor(factor)``: while it is entered on this thread, the launches below that read
+# gradients (prepare, AdamW, 8-bit AdamW) multiply each by ``factor[0]``, an fp32 device tensor,
+# as they read it.
+@contextlib.contextmanager
+def gradient_factor(factor):
+    saved = _factor()
+    _tls.factor = factor
+    try:
+        yield factor
+    finally:
+        _tls.factor = saved
+
+
+def _factor():
+    return getattr(_tls, "factor", None)
 
 
 # Multicast addresses of the parameters this process updates, registered by a
@@ -120,7 +138,13 @@ def muon_prepare(items, beta: float, nesterov: bool) -> None:
     rec = _recorder()
     if rec is not None:
         hdr = _lib.PrepareRecord(float(f32(beta)), float(f32(1.0 - beta)), int(bool(nesterov)), len(items))
-        rec.launch("msr_muon_prepare_rec", hdr, arr, dev)
+        rec.launch("msr_muon_prepare_rec", hdr, arr, dev, _factor())
+        return
+    factor = _factor()
+    if factor is not None:
+        _lib.check(_lib.load().msr_muon_prepare_scaled(
+            arr, len(items), float(f32(beta)), float(f32(1.0 - beta)), int(bool(nesterov)), factor.data_ptr(),
+            stream_handle(dev)), "msr_muon_prepare_scaled")
         return
     _lib.check(_lib.load().msr_muon_prepare(arr, len(items), float(f32(beta)), float(f32(1.0 - beta)),
                                             int(bool(nesterov)), stream_handle(dev)), "msr_muon_prepare")
@@ -169,7 +193,12 @@ def adamw_sr(items, lr: float, beta1: float, beta2: float, eps: float, weight_de
     dev = items[0][0].device
     rec = _recorder()
     if rec is not None:
-        rec.launch("msr_adamw_sr_rec", _lib.AdamWRecord(hp, len(items), 0), arr, dev)
+        rec.launch("msr_adamw_sr_rec", _lib.AdamWRecord(hp, len(items), 0), arr, dev, _factor())
+        return
+    factor = _factor()
+    if factor is not None:
+        _lib.check(_lib.load().msr_adamw_sr_scaled(arr, len(items), ctypes.byref(hp), factor.data_ptr(),
+                                                   stream_handle(dev)), "msr_adamw_sr_scaled")
         return
     _lib.check(_lib.load().msr_adamw_sr(arr, len(items), ctypes.byref(hp), stream_handle(dev)), "msr_adamw_sr")
 
@@ -216,6 +245,11 @@ def adamw8bit(items, qmap1, qmap2, lr, beta1, beta2, eps, weight_decay, block_si
                            float(f32(1.0 - lr * weight_decay)), int(block_size),
                            qtables.data_ptr() if qtables is not None else None)
     dev = items[0][0].device
+    factor = _factor()
+    if factor is not None:
+        _lib.check(_lib.load().msr_adamw8bit_scaled(arr, len(items), _ptr(qmap1), _ptr(qmap2), ctypes.byref(hp),
+                                                    factor.data_ptr(), stream_handle(dev)), "msr_adamw8bit_scaled")
+        return
     _lib.check(_lib.load().msr_adamw8bit(arr, len(items), _ptr(qmap1), _ptr(qmap2), ctypes.byref(hp),
                                          stream_handle(dev)), "msr_adamw8bit")
 
@@ -318,6 +352,141 @@ def centralize(grad: torch.Tensor, centralization: float) -> torch.Tensor:
                                                float(centralization), stream_handle(g.device)),
                "msr_centralize_bf16")
     return out
+
+
+# ---------------------------------------------------------------------------------------
+# Gradient norm and clipping
+# ---------------------------------------------------------------------------------------
+GRAD_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+NORM_TYPES = {math.inf: 0, 1.0: 1, 2.0: 2}
+
+
+def is_dense(t: torch.Tensor) -> bool:
+    """Whether the elements of ``t`` fill one stretch of memory, in whatever order."""
+    if t.is_contiguous():
+        return True
+    size = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if st != size:
+            return False
+        size *= n
+    return True
+
+
+def _refuse_grad(g, device):
+    if g.layout is not torch.strided:
+        raise RuntimeError("gradients must not be sparse")
+    if not g.is_cuda:
+        raise ValueError("gradients must be CUDA tensors (muon_sr_b200 has no CPU path)")
+    if g.dtype not in GRAD_DTYPES:
+        raise ValueError(f"gradients must be bfloat16, float16 or float32, got {g.dtype}")
+    raise ValueError(f"gradients must be on one device, got {g.device} and cuda:{device}")
+
+
+class GradTable:
+    """Gradients as the C entries of ``msr_grad_norm`` and ``msr_grad_scale``: CUDA tensors of
+    the dtypes above on one device, mixed at will. A gradient that is not dense goes through a
+    contiguous copy, which ``grad_scale_`` copies back. ``device`` is needed where the list may
+    be empty."""
+
+    __slots__ = ("grads", "dense", "words", "device")
+
+    def __init__(self, grads, device=None):
+        self.grads = self.dense = grads
+        self.words = array.array("q")
+        if not grads:
+            self.device = torch.device(device)
+            return
+        self.device = grads[0].device
+        index = grads[0].get_device()
+        words = self.words
+        for i, g in enumerate(grads):
+            code = GRAD_DTYPES.get(g.dtype)
+            if code is None or g.layout is not torch.strided or g.get_device() != index or index < 0:
+                _refuse_grad(g, index)
+            if not g.is_contiguous() and not is_dense(g):
+                if self.dense is grads:
+                    self.dense = list(grads)
+                self.dense[i] = g = g.contiguous()
+            words.extend((g.data_ptr(), g.numel(), code))
+
+    def address(self):
+        return self.words.buffer_info()[0] if self.words else None
+
+
+class GradNorm:
+    """The norm of one set of gradients on the device (``msr_clip_state``): ``norm`` (0-dim
+    fp32) and ``factor`` (1 element, fp32) are views of ``state``."""
+
+    __slots__ = ("state", "norm", "factor", "each")
+
+    def __init__(self, device, count=None):
+        self.state = torch.empty(ctypes.sizeof(_lib.ClipState) // 4, dtype=torch.float32, device=device)
+        self.norm = self.state[2]
+        self.factor = self.state[3:4]
+        self.each = None if count is None else torch.empty(count, dtype=torch.float32, device=device)
+
+    def power(self, norm_type):
+        """The sum of powers as one fp64 value or, for the infinity norm, the largest magnitude
+        as the int64 its bits form (which orders as the values do, NaN last)."""
+        return self.state[:2].view(torch.int64 if norm_type == math.inf else torch.float64)
+
+
+@contextlib.contextmanager
+def _on(device):
+    """Launches go to the current device: make it ``device`` where it is another."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        yield
+    else:
+        with torch.cuda.device(device):
+            yield
+
+
+def grad_norm(table: GradTable, norm_type: float = 2.0, scale: float = 1.0, max_norm: float = math.inf,
+              per_tensor: bool = False) -> GradNorm:
+    """The norm of all gradients of ``table`` together times ``scale``, the factor that clips it
+    to ``max_norm`` and, with ``per_tensor``, the norm of each. The workspace belongs to this
+    call, so calls on several streams or in several captured graphs never share one."""
+    count, device = len(table.grads), table.device
+    lib = _lib.load()
+    nbytes = lib.msr_grad_norm_workspace_bytes(count)
+    out = GradNorm(device, count if per_tensor else None)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    rec = _recorder()
+    if rec is not None:
+        rec.constant("gradient norm", (norm_type, scale, max_norm, count))
+        if not rec.launches:
+            return out
+        for t in (out.state, ws, *table.dense):
+            rec.hold(t)
+    with _on(device):
+        _lib.check(lib.msr_grad_norm(
+            table.address(), count, NORM_TYPES[norm_type], scale, max_norm, out.state.data_ptr(),
+            out.each.data_ptr() if out.each is not None else None, ws.data_ptr(), nbytes, stream_handle(device)),
+            "msr_grad_norm")
+    return out
+
+
+def grad_factor(norm: GradNorm, norm_type: float, scale: float, max_norm: float) -> None:
+    """Norm and factor again from ``norm.power``, which the caller has combined over ranks."""
+    device = norm.state.device
+    with _on(device):
+        _lib.check(_lib.load().msr_grad_factor(norm.state.data_ptr(), NORM_TYPES[norm_type], scale, max_norm,
+                                               stream_handle(device)), "msr_grad_factor")
+
+
+def grad_scale_(table: GradTable, norm: GradNorm) -> None:
+    """Multiply the gradients by ``norm.factor`` in place; nothing is written where clipping has
+    nothing to do."""
+    if not table.grads:
+        return
+    with _on(table.device):
+        _lib.check(_lib.load().msr_grad_scale(table.address(), len(table.grads), norm.state.data_ptr(),
+                                              stream_handle(table.device)), "msr_grad_scale")
+    if table.dense is not table.grads:
+        for g, d in zip(table.grads, table.dense):
+            if g is not d:
+                g.copy_(d)
 
 
 SR_NOISE_MODES = {"reference": 0, "fast": 1, "none": 2}

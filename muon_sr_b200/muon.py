@@ -19,6 +19,7 @@ import contextlib
 import torch
 from torch.optim import Optimizer
 
+from . import clipping
 from . import kernels as K
 from . import staging
 from .adamw import adamw_group_step
@@ -367,6 +368,19 @@ class _MuonBase(Optimizer):
 
     _random_seeds = False   # True: seeds from torch's generator (MuonSR classes)
     _record_step = True     # False: no "step" in the Muon state (MuonSR classes)
+    grad_norm = None        # the last step's gradient norm, where it clipped
+
+    @torch.no_grad()
+    def step(self, closure=None, max_norm=None, grad_scale=1.0):
+        """One step; ``max_norm`` and ``grad_scale`` clip the gradients by their global norm as
+        the updates read them (see ``clipping``)."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        with clipping.clipped_step(self, max_norm, grad_scale):
+            self._update()
+        return loss
 
     def _setup(self, shard):
         self._shard = shard
@@ -444,12 +458,7 @@ class TritonMuonSR(_MuonBase):
                                       ns_steps=ns_steps, batch_ns=batch_ns))
         self._setup(shard)
 
-    @torch.no_grad()
-    def step(self, closure=None):
-        loss = None
-        if closure is not None:
-            with torch.enable_grad():
-                loss = closure()
+    def _update(self):
         if self._shard:
             self._shard.bind(self)
         seeder = _Seeder(self._random_seeds)
@@ -458,7 +467,6 @@ class TritonMuonSR(_MuonBase):
             self._run_muon_group(gi, group, group["batch_ns"], batched_groups, seeder)
         if self._shard:
             self._shard.sync_params(self)
-        return loss
 
 
 class MuonSR(TritonMuonSR):
@@ -492,12 +500,7 @@ class TritonMuonSRWithAuxAdam(_MuonBase):
         super().__init__(param_groups, {})
         self._setup(shard)
 
-    @torch.no_grad()
-    def step(self, closure=None):
-        loss = None
-        if closure is not None:
-            with torch.enable_grad():
-                loss = closure()
+    def _update(self):
         sh = self._shard
         if sh:
             sh.bind(self)
@@ -547,7 +550,6 @@ class TritonMuonSRWithAuxAdam(_MuonBase):
         run_deferred()
         if sh:
             sh.sync_params(self)
-        return loss
 
 
 class MuonSRWithAuxAdam(TritonMuonSRWithAuxAdam):

@@ -307,6 +307,21 @@ class Sharder:
             own.copy_(mine / self.world if average else mine)
         return {"chunk_elements": chunk, "padding": lay["padding"], "tensors": len(params)}
 
+    def owned(self, params):
+        """Those of ``params`` whose update is this rank's (after ``reduce_grads`` or a step has
+        assigned them)."""
+        if self._owner is None or any(id(p) not in self._owner for p in params):
+            raise RuntimeError("the sharder has not assigned these parameters: call reduce_grads(optimizer) first")
+        return [p for p in params if self._owner[id(p)] == self.rank]
+
+    def combine_power(self, power):
+        """Collective: ``power`` (one element, the share of this rank's gradients in a global
+        norm) becomes the sum over the ranks or, for the bits of a largest magnitude (int64),
+        the maximum."""
+        if self.world > 1:
+            op = dist.ReduceOp.SUM if power.is_floating_point() else dist.ReduceOp.MAX
+            dist.all_reduce(power, op=op, group=self.group)
+
     def _pack_layout(self, params, key):
         """Owner-ordered slots of the packed gradient buffer (same on every rank)."""
         align = 64  # elements: 128-byte slots keep every gradient 16-byte aligned

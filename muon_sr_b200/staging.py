@@ -176,7 +176,11 @@ class HostStaging:
                 self._downloaded.add(i)
 
     # ---- the step ----
-    def step(self):
+    def step(self, max_norm=None, grad_scale=1.0):
+        """One step. With ``max_norm`` it clips the gradients by their global norm as
+        ``optimizer.step(max_norm=, grad_scale=)`` does: the norm has to be known before the
+        first update, so all uploads then come before it and overlap only one another."""
+        clip = {} if max_norm is None and grad_scale == 1.0 else dict(max_norm=max_norm, grad_scale=grad_scale)
         if getattr(_tls, "io", None) is not None:
             raise RuntimeError("HostStaging steps do not nest")
         cur = torch.cuda.current_stream(self._device)
@@ -192,7 +196,7 @@ class HostStaging:
         self.d2h_bytes = 0
         _tls.io = self
         try:
-            loss = self.optimizer.step()
+            loss = self.optimizer.step(**clip)
         finally:
             _tls.io = None
         for s in (self._up, self._down):
