@@ -278,7 +278,9 @@ int msr_adamw8bit(const msr_adamw8bit_entry* entries, int count, const float* qm
  * msr_grad_scale multiplies every entry by state->factor in place, in fp32, rounded to nearest
  * even; when state->active is 0 it leaves them untouched. Entries of one call must not share
  * memory (MSR_ERR_INVALID). An entry may start at any multiple of its element size; entries of
- * numel 0 may have a NULL pointer. */
+ * numel 0 may have a NULL pointer.
+ * msr_grad_clip is msr_grad_norm followed by msr_grad_scale, in fewer launches: one for sets of
+ * up to 512 KB, two otherwise (up to 512 entries). */
 enum msr_dtype { MSR_BF16 = 0, MSR_FP16 = 1, MSR_FP32 = 2 };
 enum msr_norm { MSR_NORM_INF = 0, MSR_NORM_1 = 1, MSR_NORM_2 = 2 };
 
@@ -307,6 +309,9 @@ int msr_grad_factor(msr_clip_state* state, int norm, double scale, double max_no
 
 int msr_grad_scale(const msr_grad_entry* entries, int count, const msr_clip_state* state,
                    msr_stream_t stream);
+
+int msr_grad_clip(const msr_grad_entry* entries, int count, int norm, double scale, double max_norm,
+                  msr_clip_state* state, void* workspace, size_t workspace_bytes, msr_stream_t stream);
 
 /* The updates above with every gradient read as g * grad_factor[0], an fp32 scalar in device
  * memory (state->factor of msr_grad_norm): the product is taken in fp32 and is not rounded to

@@ -44,7 +44,6 @@ def _refuse_nonfinite(norm, norm_type):
                            "clipped. Pass error_if_nonfinite=False to clip with the non-finite norm anyway.")
 
 
-@torch.no_grad()
 def get_total_norm(tensors, norm_type=2.0, error_if_nonfinite=False, *, per_tensor=False):
     """The norm of ``tensors`` (bf16, fp16 or fp32 CUDA tensors on one device, mixed at will) as
     one vector: a 0-dim fp32 tensor on their device, 0 for an empty list.
@@ -72,7 +71,6 @@ def _norm_over_ranks(table, norm_type, grad_scale, max_norm, shard):
     return norm
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, *, grad_scale=1.0, shard=None):
     """Multiply the gradients of ``parameters`` in place by
     ``grad_scale * min(1, max_norm / (norm + 1e-6))``, ``norm`` being the norm of all of them
@@ -94,21 +92,14 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     whose gradients share memory are refused."""
     norm_type = _norm_type(norm_type)
     max_norm, grad_scale = _bounds(max_norm, grad_scale)
-    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(dict.fromkeys(parameters))
-    params = [p for p in parameters if p.grad is not None]
-    device = _device(params)
-    if shard is not None:
-        params = shard.owned(params)
-    if device is None:
-        if shard is None:
-            return torch.zeros(())
-        device = torch.device("cuda", torch.cuda.current_device())
-    grads = [p.grad for p in params]
-    for g in grads:
-        if g.layout is torch.strided and not g.is_contiguous() and \
-                any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
-            raise ValueError("gradients must not be expanded tensors: their elements share memory")
-    table = K.GradTable(grads, device)
+    table = _gradients([parameters] if isinstance(parameters, torch.Tensor) else parameters, shard)
+    if table is None:
+        return torch.zeros(())
+    if table.dense is not table.grads and any(st == 0 and n > 1 for g in table.grads
+                                              for st, n in zip(g.stride(), g.shape)):
+        raise ValueError("gradients must not be expanded tensors: their elements share memory")
+    if shard is None and not error_if_nonfinite:
+        return K.grad_clip_(table, norm_type, grad_scale, max_norm).norm
     norm = _norm_over_ranks(table, norm_type, grad_scale, max_norm, shard)
     if error_if_nonfinite:
         _refuse_nonfinite(norm.norm, norm_type)
@@ -116,8 +107,20 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     return norm.norm
 
 
-def _device(params):
-    return params[0].grad.device if params else None
+def _gradients(parameters, shard):
+    """The ``GradTable`` of the parameters that have a gradient, each once (with a sharder: those
+    of them that this rank owns), or None where there is nothing to launch."""
+    parameters = list(parameters)
+    grads = [g for p in parameters if (g := p.grad) is not None]
+    if shard is not None or staging.active() or len(set(map(id, grads))) < len(grads):
+        params = list({id(p): p for p in parameters if p.grad is not None}.values())
+        if shard is not None:
+            params = shard.owned(params)
+        staging.need(params)
+        grads = [p.grad for p in params]
+    if not grads and shard is None:
+        return None
+    return K.GradTable(grads, None if grads else torch.cuda.current_device())
 
 
 def clipped_step(optimizer, max_norm, grad_scale):
@@ -130,18 +133,12 @@ def clipped_step(optimizer, max_norm, grad_scale):
             raise ValueError("grad_scale needs max_norm (math.inf clips nothing)")
         return contextlib.nullcontext()
     max_norm, grad_scale = _bounds(max_norm, grad_scale)
-    params = list(dict.fromkeys(p for g in optimizer.param_groups for p in g["params"] if p.grad is not None))
-    device = _device(params)
     shard = getattr(optimizer, "_shard", None)
     if shard is not None:
         shard._ensure(optimizer)
-        params = shard.owned(params)
-    if device is None:
-        if shard is None:
-            return contextlib.nullcontext()
-        device = torch.device("cuda", torch.cuda.current_device())
-    staging.need(params)
-    table = K.GradTable([p.grad for p in params], device)
+    table = _gradients([p for g in optimizer.param_groups for p in g["params"]], shard)
+    if table is None:
+        return contextlib.nullcontext()
     norm = _norm_over_ranks(table, 2.0, grad_scale, max_norm, shard)
     optimizer.grad_norm = norm.norm
     return K.gradient_factor(norm.factor)

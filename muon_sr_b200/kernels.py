@@ -8,7 +8,9 @@ reference's kernels see them.
 import array
 import contextlib
 import ctypes
+import itertools
 import math
+import operator
 import threading
 
 import numpy as np
@@ -373,58 +375,73 @@ def is_dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _refuse_grad(g, device):
-    if g.layout is not torch.strided:
-        raise RuntimeError("gradients must not be sparse")
-    if not g.is_cuda:
-        raise ValueError("gradients must be CUDA tensors (muon_sr_b200 has no CPU path)")
-    if g.dtype not in GRAD_DTYPES:
-        raise ValueError(f"gradients must be bfloat16, float16 or float32, got {g.dtype}")
-    raise ValueError(f"gradients must be on one device, got {g.device} and cuda:{device}")
+# Read off many tensors by ``map``: a fraction of the time of a loop in Python, which for a few
+# hundred gradients would take longer than their norm.
+_data_ptr, _numel_of, _device_index, _is_contiguous = (
+    torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous)
+_dtype_of = operator.attrgetter("dtype")
+
+
+def _refuse_grads(grads):
+    """Raise for the first of ``grads`` that a ``GradTable`` cannot hold."""
+    for g in grads:
+        if g.layout is not torch.strided:
+            raise RuntimeError("gradients must not be sparse")
+        if not g.is_cuda:
+            raise ValueError("gradients must be CUDA tensors (muon_sr_b200 has no CPU path)")
+        if g.dtype not in GRAD_DTYPES:
+            raise ValueError(f"gradients must be bfloat16, float16 or float32, got {g.dtype}")
+        if g.device != grads[0].device:
+            raise ValueError(f"gradients must be on one device, got {grads[0].device} and {g.device}")
 
 
 class GradTable:
     """Gradients as the C entries of ``msr_grad_norm`` and ``msr_grad_scale``: CUDA tensors of
     the dtypes above on one device, mixed at will. A gradient that is not dense goes through a
-    contiguous copy, which ``grad_scale_`` copies back. ``device`` is needed where the list may
-    be empty."""
+    contiguous copy, which ``grad_scale_`` copies back. ``device`` (an index) is needed where the
+    list may be empty."""
 
-    __slots__ = ("grads", "dense", "words", "device")
+    __slots__ = ("grads", "dense", "words", "index")
 
     def __init__(self, grads, device=None):
         self.grads = self.dense = grads
-        self.words = array.array("q")
         if not grads:
-            self.device = torch.device(device)
+            self.words, self.index = array.array("q"), device
             return
-        self.device = grads[0].device
-        index = grads[0].get_device()
-        words = self.words
-        for i, g in enumerate(grads):
-            code = GRAD_DTYPES.get(g.dtype)
-            if code is None or g.layout is not torch.strided or g.get_device() != index or index < 0:
-                _refuse_grad(g, index)
-            if not g.is_contiguous() and not is_dense(g):
-                if self.dense is grads:
-                    self.dense = list(grads)
-                self.dense[i] = g = g.contiguous()
-            words.extend((g.data_ptr(), g.numel(), code))
+        self.index = grads[0].get_device()
+        codes = list(map(GRAD_DTYPES.get, map(_dtype_of, grads)))
+        if self.index < 0 or None in codes or len(set(map(_device_index, grads))) > 1:
+            _refuse_grads(grads)
+        try:
+            if not all(map(_is_contiguous, grads)):
+                self.dense = [g if is_dense(g) else g.contiguous() for g in grads]
+            self.words = array.array("q", itertools.chain.from_iterable(
+                zip(map(_data_ptr, self.dense), map(_numel_of, self.dense), codes)))
+        except RuntimeError:  # a sparse tensor has neither strides nor a pointer
+            _refuse_grads(grads)
+            raise
 
     def address(self):
         return self.words.buffer_info()[0] if self.words else None
 
 
 class GradNorm:
-    """The norm of one set of gradients on the device (``msr_clip_state``): ``norm`` (0-dim
-    fp32) and ``factor`` (1 element, fp32) are views of ``state``."""
+    """The norm of one set of gradients on the device: ``state`` holds the fields of
+    ``msr_clip_state``, ``each`` the norms of the tensors if they were asked for."""
 
-    __slots__ = ("state", "norm", "factor", "each")
+    __slots__ = ("state", "each")
 
     def __init__(self, device, count=None):
         self.state = torch.empty(ctypes.sizeof(_lib.ClipState) // 4, dtype=torch.float32, device=device)
-        self.norm = self.state[2]
-        self.factor = self.state[3:4]
         self.each = None if count is None else torch.empty(count, dtype=torch.float32, device=device)
+
+    @property
+    def norm(self):
+        return self.state[2]
+
+    @property
+    def factor(self):
+        return self.state[3:4]
 
     def power(self, norm_type):
         """The sum of powers as one fp64 value or, for the infinity norm, the largest magnitude
@@ -432,14 +449,16 @@ class GradNorm:
         return self.state[:2].view(torch.int64 if norm_type == math.inf else torch.float64)
 
 
-@contextlib.contextmanager
-def _on(device):
-    """Launches go to the current device: make it ``device`` where it is another."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        yield
-    else:
-        with torch.cuda.device(device):
-            yield
+def _launch(index, name, *args):
+    """Call entry point ``name`` with ``args`` and the current stream of device ``index``,
+    which is made the current device for the call where it is another."""
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return _launch(index, name, *args)
+    # (the raw handle: a Stream object around it would cost more than the launch)
+    status = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, name)
 
 
 def grad_norm(table: GradTable, norm_type: float = 2.0, scale: float = 1.0, max_norm: float = math.inf,
@@ -447,11 +466,10 @@ def grad_norm(table: GradTable, norm_type: float = 2.0, scale: float = 1.0, max_
     """The norm of all gradients of ``table`` together times ``scale``, the factor that clips it
     to ``max_norm`` and, with ``per_tensor``, the norm of each. The workspace belongs to this
     call, so calls on several streams or in several captured graphs never share one."""
-    count, device = len(table.grads), table.device
-    lib = _lib.load()
-    nbytes = lib.msr_grad_norm_workspace_bytes(count)
-    out = GradNorm(device, count if per_tensor else None)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    count, index = len(table.grads), table.index
+    nbytes = _lib.load().msr_grad_norm_workspace_bytes(count)
+    out = GradNorm(index, count if per_tensor else None)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=index)
     rec = _recorder()
     if rec is not None:
         rec.constant("gradient norm", (norm_type, scale, max_norm, count))
@@ -459,34 +477,42 @@ def grad_norm(table: GradTable, norm_type: float = 2.0, scale: float = 1.0, max_
             return out
         for t in (out.state, ws, *table.dense):
             rec.hold(t)
-    with _on(device):
-        _lib.check(lib.msr_grad_norm(
-            table.address(), count, NORM_TYPES[norm_type], scale, max_norm, out.state.data_ptr(),
-            out.each.data_ptr() if out.each is not None else None, ws.data_ptr(), nbytes, stream_handle(device)),
-            "msr_grad_norm")
+    _launch(index, "msr_grad_norm", table.address(), count, NORM_TYPES[norm_type], scale, max_norm,
+            out.state.data_ptr(), None if out.each is None else out.each.data_ptr(), ws.data_ptr(), nbytes)
     return out
 
 
 def grad_factor(norm: GradNorm, norm_type: float, scale: float, max_norm: float) -> None:
     """Norm and factor again from ``norm.power``, which the caller has combined over ranks."""
-    device = norm.state.device
-    with _on(device):
-        _lib.check(_lib.load().msr_grad_factor(norm.state.data_ptr(), NORM_TYPES[norm_type], scale, max_norm,
-                                               stream_handle(device)), "msr_grad_factor")
+    _launch(norm.state.get_device(), "msr_grad_factor", norm.state.data_ptr(), NORM_TYPES[norm_type], scale, max_norm)
 
 
 def grad_scale_(table: GradTable, norm: GradNorm) -> None:
     """Multiply the gradients by ``norm.factor`` in place; nothing is written where clipping has
     nothing to do."""
-    if not table.grads:
-        return
-    with _on(table.device):
-        _lib.check(_lib.load().msr_grad_scale(table.address(), len(table.grads), norm.state.data_ptr(),
-                                              stream_handle(table.device)), "msr_grad_scale")
+    if table.grads:
+        _launch(table.index, "msr_grad_scale", table.address(), len(table.grads), norm.state.data_ptr())
+        _copy_back(table)
+
+
+def grad_clip_(table: GradTable, norm_type: float, scale: float, max_norm: float) -> GradNorm:
+    """``grad_norm`` and ``grad_scale_`` in fewer launches."""
+    count, index = len(table.grads), table.index
+    nbytes = _lib.load().msr_grad_norm_workspace_bytes(count)
+    out = GradNorm(index)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=index)
+    _launch(index, "msr_grad_clip", table.address(), count, NORM_TYPES[norm_type], scale, max_norm,
+            out.state.data_ptr(), ws.data_ptr(), nbytes)
+    _copy_back(table)
+    return out
+
+
+def _copy_back(table):
     if table.dense is not table.grads:
-        for g, d in zip(table.grads, table.dense):
-            if g is not d:
-                g.copy_(d)
+        with torch.no_grad():
+            for g, d in zip(table.grads, table.dense):
+                if g is not d:
+                    g.copy_(d)
 
 
 SR_NOISE_MODES = {"reference": 0, "fast": 1, "none": 2}

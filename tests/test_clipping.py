@@ -71,13 +71,15 @@ def test_c_argument_errors():
 
     def norm(words=(ptr, 4, 0), count=1, kind=2, scale=1.0, bound=1.0, state=ptr, ws=ptr, size=need):
         arr = (ctypes.c_int64 * 3)(*words)
-        return lib.msr_grad_norm(arr, count, kind, scale, bound, state, None, ws, size, None)
+        st = lib.msr_grad_norm(arr, count, kind, scale, bound, state, None, ws, size, None)
+        assert lib.msr_grad_clip(arr, count, kind, scale, bound, state, ws, size, None) == st
+        return st
     for kw in (dict(count=-1), dict(kind=3), dict(kind=-1), dict(scale=0.0), dict(scale=math.inf),
                dict(scale=math.nan), dict(bound=-1.0), dict(bound=math.nan), dict(state=None), dict(state=ptr + 4),
                dict(ws=None), dict(ws=ptr + 4), dict(words=(0, 4, 0)), dict(words=(ptr, -1, 0)),
                dict(words=(ptr, 4, 3)), dict(words=(ptr + 1, 4, 0)), dict(words=(ptr + 2, 4, 2))):
         assert norm(**kw) == 1, kw
-        assert lib.msr_last_error().startswith(b"msr_grad_norm")
+        assert lib.msr_last_error().startswith(b"msr_grad_clip")
     assert norm(size=need - 1) == 4
     assert lib.msr_grad_norm(None, 1, 2, 1.0, 1.0, ptr, None, ptr, need, None) == 1
     assert lib.msr_grad_factor(None, 2, 1.0, 1.0, None) == 1
@@ -111,16 +113,17 @@ def test_state_layout():
 
 def _fake_kernels():
     """The kernels' formulas on CPU tensors, in place of the launches."""
-    def table(grads, device=None):
-        return [g for g in grads]
+    class Table:
+        def __init__(self, grads, device=None):
+            self.grads = self.dense = grads
 
     def put(out, kind, scale, bound, power):
         norm = (math.sqrt(power) if kind == 2.0 else power) * scale
         out.norm.fill_(norm)
         out.factor.fill_(scale * min(1.0, bound / (norm + 1e-6)) if bound != math.inf else scale)
 
-    def grad_norm(grads, kind, scale, bound):
-        out = K.GradNorm("cpu")
+    def grad_norm(table, kind, scale, bound):
+        grads, out = table.grads, K.GradNorm("cpu")
         each = [float(g.double().abs().max()) if kind == math.inf else float((g.double().abs() ** kind).sum())
                 for g in grads]
         power = max(each, default=0.0) if kind == math.inf else sum(each)
@@ -131,10 +134,10 @@ def _fake_kernels():
     def factor(out, kind, scale, bound):
         put(out, kind, scale, bound, out.state[:2].view(torch.float64).item())
 
-    def scale(grads, out):
-        for g in grads:
+    def scale(table, out):
+        for g in table.grads:
             g.mul_(out.factor.to(g.dtype))
-    K.GradTable, K.grad_norm, K.grad_factor, K.grad_scale_ = table, grad_norm, factor, scale
+    K.GradTable, K.grad_norm, K.grad_factor, K.grad_scale_ = Table, grad_norm, factor, scale
 
 
 def _shard_worker(rank, world, port, out):
@@ -196,7 +199,7 @@ def test_sharded_norm_two_ranks_gloo():
     procs = [ctx.Process(target=_shard_worker, args=(r, 2, port, q)) for r in range(2)]
     for p in procs:
         p.start()
-    got = sorted(q.get(timeout=120) for _ in procs)
+    got = sorted(q.get(timeout=60) for _ in procs)
     for p in procs:
         p.join(timeout=60)
         assert p.exitcode == 0
