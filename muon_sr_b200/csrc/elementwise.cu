@@ -26,13 +26,13 @@ constexpr int EW_ITERS = 2;
 constexpr int64_t EW_CHUNK = EW_THREADS * EW_VEC * EW_ITERS;  // 4096 elements
 constexpr int MAXE = 64;
 constexpr int EW_BLOCKS_PER_SM = 4;
-// AdamW: the three Philox chains of each element need more than 64 registers. Measured on 2^30
-// elements with the reference noise: 1 vector of 8 per thread and chunk at 2 CTAs per SM
-// (122 registers, no spills) 1645 GB/s; 2 vectors at 2 CTAs per SM (128 registers, 40 bytes
-// of spills) 1490; 1 vector at 3 or 4 CTAs per SM (80 / 64 registers, spilling) slower still.
+// AdamW: the three Philox chains of each element need more than 64 registers, and the kernel is
+// bound by their multiplies. One CTA of 512 threads per SM, one vector of 8 per thread and chunk,
+// the noise of a chunk drawn between its loads and their first use (see the kernel).
+constexpr int ADAMW_THREADS = 512;
 constexpr int ADAMW_ITERS = 1;
-constexpr int ADAMW_MINB = 2;
-constexpr int64_t ADAMW_CHUNK = EW_THREADS * EW_VEC * ADAMW_ITERS;
+constexpr int ADAMW_MINB = 1;
+constexpr int64_t ADAMW_CHUNK = ADAMW_THREADS * EW_VEC * ADAMW_ITERS;
 // Apply: one vector per thread and chunk (60 registers, no spills) measured 2350 GB/s on 2^30
 // elements against 2262 for two vectors (64 registers with 20 bytes of spills).
 constexpr int APPLY_ITERS = 1;
@@ -422,13 +422,13 @@ __device__ __forceinline__ void adamw_tail(const AdamWArgs& a, const msr_adamw_e
 
 // ITERS vectors of 8 elements per thread and chunk; MINB CTAs per SM for the register budget.
 template <int ITERS, int MINB, int NOISE, bool REC, bool SCALED>
-__global__ __launch_bounds__(EW_THREADS, MINB) void adamw_kernel(const __grid_constant__ AdamWArgs a) {
-  constexpr bool FAST = NOISE == NOISE_FAST;
+__global__ __launch_bounds__(ADAMW_THREADS, MINB) void adamw_kernel(const __grid_constant__ AdamWArgs a) {
   const float gs = SCALED ? *a.gscale : 1.f;
-  constexpr int64_t CHUNK = EW_THREADS * EW_VEC * ITERS;
+  constexpr int64_t CHUNK = ADAMW_THREADS * EW_VEC * ITERS;
   const int64_t total = a.prefix[a.count];
+  int ei = find_entry<MAXE>(a.prefix, a.count, blockIdx.x);
   for (int64_t chunk = blockIdx.x; chunk < total; chunk += gridDim.x) {
-    const int ei = find_entry<MAXE>(a.prefix, a.count, chunk);
+    while (a.prefix[ei + 1] <= chunk) ++ei;  // chunks only move forward; prefix[count] = total
     const msr_adamw_entry& E = entry_of<REC>(a, ei);
     uint16_t* p = static_cast<uint16_t*>(E.param);
     uint16_t* pm = static_cast<uint16_t*>(E.param_mc);  // multicast weights (sharded steps)
@@ -443,7 +443,7 @@ __global__ __launch_bounds__(EW_THREADS, MINB) void adamw_kernel(const __grid_co
       U16x8 vp[ITERS], vg[ITERS], vm[ITERS], vv[ITERS];
 #pragma unroll
       for (int it = 0; it < ITERS; ++it) {
-        const int64_t idx = base + (int64_t)(it * EW_THREADS + threadIdx.x) * EW_VEC;
+        const int64_t idx = base + (int64_t)(it * ADAMW_THREADS + threadIdx.x) * EW_VEC;
         if (idx + EW_VEC <= n) {
           vp[it] = ld_u16x8(p + idx);
           vg[it] = ld_u16x8_stream(g + idx);
@@ -453,21 +453,23 @@ __global__ __launch_bounds__(EW_THREADS, MINB) void adamw_kernel(const __grid_co
       }
 #pragma unroll
       for (int it = 0; it < ITERS; ++it) {
-        const int64_t idx = base + (int64_t)(it * EW_THREADS + threadIdx.x) * EW_VEC;
+        const int64_t idx = base + (int64_t)(it * ADAMW_THREADS + threadIdx.x) * EW_VEC;
         if (idx + EW_VEC <= n) {
+          // All noise of the vector before the first use of what is being loaded: the chains need
+          // only the counters, and kept as 16-bit halves they cost fewer registers than chains
+          // running beside the update. 2^30 elements: 1760 GB/s, against 1645 with the noise drawn
+          // where each rounding needs it and 2 CTAs of 256 threads. (Giving each CTA consecutive
+          // chunks, to keep an entry's round keys across them, spills: 1744.)
           uint32_t rm[EW_VEC], rv[EW_VEC], rp[EW_VEC];
-          if (FAST) {
-            nm.eight(static_cast<uint64_t>(idx), rm);
-            nv.eight(static_cast<uint64_t>(idx), rv);
-            np_.eight(static_cast<uint64_t>(idx), rp);
-          }
+          nm.eight(static_cast<uint64_t>(idx), rm);
+          nv.eight(static_cast<uint64_t>(idx), rv);
 #pragma unroll
-          for (int j = 0; j < EW_VEC; ++j) {
-            const uint64_t c = static_cast<uint64_t>(idx + j);
-            adamw_one<NOISE, SCALED>(vp[it].v[j], vg[it].v[j], gs, vm[it].v[j], vv[it].v[j], hp_of<REC>(a), ss, bc2s, [&](int w) {
-              return w == 0 ? (FAST ? rm[j] : nm.at(c)) : w == 1 ? (FAST ? rv[j] : nv.at(c)) : (FAST ? rp[j] : np_.at(c));
-            });
-          }
+          for (int j = 0; j < EW_VEC; ++j) rm[j] = (rm[j] & 0xFFFFu) | (rv[j] << 16);
+          np_.eight(static_cast<uint64_t>(idx), rp);
+#pragma unroll
+          for (int j = 0; j < EW_VEC; ++j)
+            adamw_one<NOISE, SCALED>(vp[it].v[j], vg[it].v[j], gs, vm[it].v[j], vv[it].v[j], hp_of<REC>(a), ss, bc2s,
+                                     [&](int w) { return w == 0 ? rm[j] : w == 1 ? rm[j] >> 16 : rp[j]; });
           if (pm)
             mc_st_u16x8(pm + idx, vp[it]);
           else
@@ -483,7 +485,7 @@ __global__ __launch_bounds__(EW_THREADS, MINB) void adamw_kernel(const __grid_co
       adamw_tail<NOISE, REC, SCALED>(a, E, gs, nm, nv, np_, lo, lo + ITERS * EW_VEC < n ? lo + ITERS * EW_VEC : n);
     } else {
       for (int it = 0; it < ITERS * EW_VEC; ++it) {
-        const int64_t i = base + it * EW_THREADS + threadIdx.x;
+        const int64_t i = base + it * ADAMW_THREADS + threadIdx.x;
         if (i < n) {
           uint16_t pb = p[i], mb = m[i], vb = v[i];
           adamw_one<NOISE, SCALED>(pb, g[i], gs, mb, vb, hp_of<REC>(a), ss, bc2s, [&](int w) {
@@ -689,7 +691,7 @@ int adamw_launch(const msr_adamw_entry* entries, int count, const msr_adamw_hpar
     // one wave of resident CTAs (ADAMW_MINB per SM), each walking its chunks
     const int64_t cap = static_cast<int64_t>(sm_count()) * ADAMW_MINB;
     const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(chunks, cap)));
-    kern<<<grid, EW_THREADS, 0, to_stream(stream)>>>(a);
+    kern<<<grid, ADAMW_THREADS, 0, to_stream(stream)>>>(a);
     int st = check_launch("adamw_kernel");
     if (st) return st;
   }

@@ -11,6 +11,7 @@ import ctypes
 import itertools
 import math
 import operator
+import struct
 import threading
 
 import numpy as np
@@ -175,21 +176,25 @@ def muon_apply(items, lr: float, weight_decay: float) -> None:
                                           stream_handle(dev)), "msr_muon_apply")
 
 
+_ADAMW_ENTRY = struct.Struct("=4Qq3Q2fQ")  # the fields of _lib.AdamWEntry in order
+assert _ADAMW_ENTRY.size == ctypes.sizeof(_lib.AdamWEntry)
+
+
 def adamw_sr(items, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float) -> None:
     """items: iterable of (param, grad, exp_avg, exp_avg_sq, step, seed)."""
     items = list(items)
     if not items:
         return
     arr = (_lib.AdamWEntry * len(items))()
-    for e, (p, g, m, v, step, seed) in zip(arr, items):
-        e.param, e.grad, e.exp_avg, e.exp_avg_sq = p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr()
-        e.numel = p.numel()
-        e.key_m, e.key_v, e.key_p = triton_key(seed, 0), triton_key(seed, 1), triton_key(seed, 2)
-        bc1 = 1.0 - beta1 ** step
-        bc2s = (1.0 - beta2 ** step) ** 0.5
-        e.step_size = float(f32(lr / bc1))
-        e.bc2_sqrt = float(f32(bc2s))
-        e.param_mc = _mc(p)
+    at, of_step, ss, bc2s = 0, None, 0.0, 0.0
+    for p, g, m, v, step, seed in items:
+        if step != of_step:  # nearly always one step for the whole group
+            of_step, ss = step, float(f32(lr / (1.0 - beta1 ** step)))
+            bc2s = float(f32((1.0 - beta2 ** step) ** 0.5))
+        # (one call per entry: assigning ctypes fields one by one takes three times as long)
+        _ADAMW_ENTRY.pack_into(arr, at, p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(),
+                               triton_key(seed, 0), triton_key(seed, 1), triton_key(seed, 2), ss, bc2s, _mc(p) or 0)
+        at += _ADAMW_ENTRY.size
     hp = _lib.AdamWHparams(float(f32(beta1)), float(f32(1.0 - beta1)), float(f32(beta2)), float(f32(1.0 - beta2)),
                            float(f32(eps)), float(f32(1.0 - lr * weight_decay)))
     dev = items[0][0].device
