@@ -834,6 +834,14 @@ def run_kernel_case(args):
             acc = torch.empty_like(p).normal_(0, 1e-3, generator=g)
             fn = lambda: K.grad_accum_(acc, gr, 1234)
             work = n * 6 / 1e9
+        elif args.kernel in ("grad_norm", "grad_clip"):
+            table = K.GradTable([gr])
+            if args.kernel == "grad_norm":
+                fn = lambda: K.grad_norm(table)
+                work = n * 2 / 1e9
+            else:  # scaled by 4 and clipped to 1 at every call: always active
+                fn = lambda: K.grad_clip_(table, 2.0, 4.0, 1.0)
+                work = n * 6 / 1e9  # read for the norm, read and written for the scaling
         elif args.kernel == "prepare":
             buf, upd = torch.zeros_like(p), torch.empty_like(p)
             fn = lambda: K.muon_prepare([(gr, buf, upd, 0, 7)], 0.95, True)
@@ -868,7 +876,8 @@ def main():
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--no-reference-gpu", action="store_true",
                     help="skip timing the reference's own GPU path (baseline/_ref) next to the engine")
-    ap.add_argument("--kernel", choices=["ns", "adamw8bit", "adamw", "prepare", "apply", "accum", "centralize"],
+    ap.add_argument("--kernel", choices=["ns", "adamw8bit", "adamw", "prepare", "apply", "accum", "centralize",
+                                         "grad_norm", "grad_clip"],
                     help="time one kernel alone (profiling cases) instead of the optimizer step")
     ap.add_argument("--small", action="store_true", help="with --kernel: the few-GB profiling size")
     ap.add_argument("--ns-shape", default=None,

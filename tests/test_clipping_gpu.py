@@ -239,6 +239,108 @@ def test_clip_within_the_bound_writes_nothing(dtype):
         assert all(same_bits(g, b) for g, b in zip(grads, before))
 
 
+@pytest.mark.parametrize("sizes", [
+    [8192] * 32, [8192] * 32 + [1], [8192] * 31 + [8193], [1] * 32, [1] * 33, [262144], [262145], [40, 8193, 100000],
+    [1 + (i * 37) % 301 for i in range(1300)],
+])
+@pytest.mark.parametrize("offset", [0, 5])
+def test_clip_and_norms_where_the_launches_change(sizes, offset):
+    """One cluster for up to 32 pieces of 16 KB, two launches up to 512 tensors, more beyond."""
+    bufs, grads = make(sizes, torch.bfloat16, seed=len(sizes), offset=offset)
+    before = [b.clone() for b in bufs]
+    for p in (2.0, 1.0, math.inf):
+        for b, old in zip(bufs, before):
+            b.copy_(old)
+        want, want_each = norm64(grads, p)
+        total, each = get_total_norm(grads, p, per_tensor=True)
+        assert_norm(total, want, p)
+        for a, b in zip(each.tolist(), want_each):
+            assert_norm(a, b, p)
+        assert_norm(clip_grad_norm_(params_of(grads), want / 2, p), want, p)
+        f = (want / 2) / (want + 1e-6)
+        assert_scaled(torch.cat(grads), torch.cat([b[offset:offset + n] for b, n in zip(before, sizes)]), f)
+        for buf, old, n in zip(bufs, before, sizes):
+            assert torch.equal(buf[:offset], old[:offset]) and torch.equal(buf[offset + n:], old[offset + n:])
+
+
+def test_clip_of_a_set_much_larger_than_the_cache():
+    sizes = [300000007, 10000001, 5, 7000000]
+    _, grads = make(sizes, torch.bfloat16, offset=3)
+    before = [g.clone() for g in grads]
+    want = math.sqrt(sum(float(torch.sum(g.double() ** 2)) for g in grads))
+    assert_norm(clip_grad_norm_(params_of(grads), want / 3), want, 2.0)
+    for g, b in zip(grads, before):
+        assert_scaled(g, b, (want / 3) / (want + 1e-6))
+
+
+@pytest.mark.parametrize("p", [2.0, 1.0, math.inf])
+def test_norm_from_the_powers_of_two_ranks(p):
+    """What a sharded norm computes: each rank's power, their sum (or maximum), norm and factor
+    from it."""
+    _, grads = make([5001, 70001, 33, 9000], torch.bfloat16)
+    want, _ = norm64(grads, p)
+    parts = [K.grad_norm(K.GradTable(g), p, 0.5, want / 8) for g in (grads[:2], grads[2:])]
+    powers = [n.power(p).clone() for n in parts]
+    both = torch.maximum(*powers) if p == math.inf else powers[0] + powers[1]
+    old = [g.clone() for g in grads]
+    for n, g in zip(parts, (grads[:2], grads[2:])):
+        n.power(p).copy_(both)
+        K.grad_factor(n, p, 0.5, want / 8)
+        assert_norm(n.norm, want / 2, p)
+        K.grad_scale_(K.GradTable(g), n)
+    for g, b in zip(grads, old):
+        assert_scaled(g, b, 0.5 * (want / 8) / (want / 2 + 1e-6))
+    none = K.grad_norm(K.GradTable([], 0), p)               # a rank that owns no gradient
+    assert float(none.norm) == 0.0
+
+
+def _one_rank(rank, port, out):
+    import os
+
+    import torch.distributed as dist
+
+    from muon_sr_b200 import Sharder
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=0, world_size=1)
+    try:
+        pa, pb = _twins()
+        oa = _hybrid(TritonMuonSRWithAuxAdam, pa)
+        sh = Sharder(transport="nccl")
+        ob = TritonMuonSRWithAuxAdam([dict(params=pb[:len(MUON)], use_muon=True, lr=0.02, weight_decay=0.01),
+                                      dict(params=pb[len(MUON):], use_muon=False, lr=3e-4, eps=1e-10)],
+                                     batch_ns=True, shard=sh)
+        for step in range(2):
+            _fill((pa, pb), 40 + step)
+            oa.step(max_norm=0.25)
+            sh.reduce_grads(ob)
+            ob.step(max_norm=0.25)
+            assert same_bits(oa.grad_norm, ob.grad_norm)
+            _assert_same(pa, pb, oa, ob, ("sharded", step))
+        na, nb = clip_grad_norm_(pa, 0.1), clip_grad_norm_(pb, 0.1, shard=sh)
+        assert float(na) == float(nb) or abs(float(na) - float(nb)) <= NORM_TOL * float(na)
+        for a, b in zip(pa, pb):
+            assert_scaled(b.grad, a.grad, 1.0)
+        out.put("ok")
+    except BaseException as e:  # the parent reports it
+        out.put(repr(e))
+        raise
+    finally:
+        dist.destroy_process_group()
+
+
+def test_sharded_clipping_on_one_rank():
+    import os
+
+    import torch.multiprocessing as mp
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    proc = ctx.Process(target=_one_rank, args=(0, 29900 + os.getpid() % 1000, q))
+    proc.start()
+    got = q.get(timeout=120)
+    proc.join(timeout=60)
+    assert got == "ok" and proc.exitcode == 0, got
+
+
 def test_clip_scale_and_bounds():
     _, grads = make([5000, 33], torch.float32)
     before = [g.clone() for g in grads]
