@@ -29,9 +29,10 @@ def adamw_group_step(state, group, offset, seed_of, owns=None, centralization=0.
     todo = []
     for i, p in enumerate(group["params"]):
         assert p.dtype == torch.bfloat16, "only bfloat16 is supported."
-        if p.grad is None:
+        g = p.grad
+        if g is None:
             continue
-        if p.grad.is_sparse:
+        if g.is_sparse:
             raise RuntimeError("TritonAdamW does not support sparse gradients")
         st = state[p]
         if not st:
@@ -41,17 +42,17 @@ def adamw_group_step(state, group, offset, seed_of, owns=None, centralization=0.
         seed = seed_of(st["step"], offset + i)
         if owns is not None and not owns(i):
             continue
-        if p.grad.dtype != torch.bfloat16:
+        if g.dtype != torch.bfloat16:
             raise ValueError("gradients must be bfloat16")
-        todo.append((p, st, seed))
+        todo.append((p, g, st, seed))
     for part in staging.batches(todo, lambda e: e[0].numel()):
-        staging.need([p for p, _, _ in part])
+        staging.need([e[0] for e in part])
         batch = []
-        for p, st, seed in part:
-            grad = K.centralize(p.grad, centralization) if centralization else p.grad.contiguous()
+        for p, g, st, seed in part:
+            grad = K.centralize(g, centralization) if centralization else g.contiguous()
             batch.append((p, grad, st["ema"], st["ema_squared"], st["step"], seed))
         K.adamw_sr(batch, group["lr"], beta1, beta2, group["eps"], group["weight_decay"])
-        staging.done([p for p, _, _ in part])
+        staging.done([e[0] for e in part])
 
 
 class TritonAdamW(Optimizer):

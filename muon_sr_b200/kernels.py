@@ -24,7 +24,11 @@ f32 = np.float32
 
 
 def stream_handle(device=None) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    index = device.index if isinstance(device, torch.device) else None
+    if index is None:
+        return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    # (the raw handle: a Stream object around it would cost half a launch)
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))
 
 
 def _require(t: torch.Tensor, name: str, dtype=torch.bfloat16):
@@ -460,7 +464,6 @@ def _launch(index, name, *args):
     if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
             return _launch(index, name, *args)
-    # (the raw handle: a Stream object around it would cost more than the launch)
     status = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _lib.check(status, name)
