@@ -153,7 +153,7 @@ __device__ __forceinline__ double power_of(float x) {
 // The power of N vectors of one thread. Sums run in fp32 over these 4 N or 8 N values and
 // join the double once: the conversions of every element would cost more than the loads. Where
 // the fp32 sum left the range in which no term can have overflowed or lost bits that count
-// (below 2^-90 a square may have underflowed: 32 terms of at most 2^-150 are 2^-55 of 2^-90),
+// (squares may underflow: 32 errors of at most 2^-150 are 2^-35 of 2^-110),
 // the same registers are summed again in double.
 template <int P, int DT, int N>
 __device__ __forceinline__ double vec_power(const uint4 (&v)[N]) {
@@ -187,7 +187,7 @@ __device__ __forceinline__ double vec_power(const uint4 (&v)[N]) {
     }
   }
   const float sum = s[0] + s[1];
-  if (sum < 0x1p126f && (P == MSR_NORM_1 || sum > 0x1p-90f)) return sum;
+  if (sum < 0x1p126f && (P == MSR_NORM_1 || sum > 0x1p-110f)) return sum;
   uint32_t any = 0u;
 #pragma unroll
   for (int i = 0; i < 4 * N; ++i) any |= w[i];

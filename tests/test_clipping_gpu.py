@@ -341,6 +341,24 @@ def test_sharded_clipping_on_one_rank():
     assert got == "ok" and proc.exitcode == 0, got
 
 
+def test_clip_mixed_types():
+    grads = sum((make([70001, 9, 300], dtype, seed=k, offset=k)[1] for k, dtype in enumerate(DTYPES)), [])
+    for some in (grads, grads[1::3]):                       # two launches, one launch
+        before = [g.clone() for g in some]
+        want, _ = norm64(some, 2.0)
+        assert_norm(clip_grad_norm_(params_of(some), want / 2), want, 2.0)
+        for g, b in zip(some, before):
+            assert_scaled(g, b, (want / 2) / (want + 1e-6))
+
+
+@pytest.mark.parametrize("std", [1e-12, 1e-16, 1e-18, 1e-22])
+def test_norm_of_tiny_gradients(std):
+    """Squares around the bottom of fp32's range, on both sides of where sums go to double."""
+    _, grads = make([40000, 77], torch.bfloat16, std=std)
+    for p in (2.0, 1.0):
+        assert_norm(get_total_norm(grads, p), norm64(grads, p)[0], p)
+
+
 def test_clip_scale_and_bounds():
     _, grads = make([5000, 33], torch.float32)
     before = [g.clone() for g in grads]
@@ -601,6 +619,19 @@ def test_step_clips_by_the_norm_of_all_groups():
             assert_scaled(opt.state[p]["ema"], p.grad, (1 - 0.9) * (want / 5) / (want + 1e-6), products=3)
     finally:
         set_sr_noise("reference")
+
+
+def test_step_clips_the_gradients_of_its_closure():
+    p = torch.nn.Parameter(torch.ones(300, dtype=torch.bfloat16, device=DEV))
+    opt = TritonAdamW([p])
+
+    def closure():
+        opt.zero_grad()
+        loss = (p.float() * 0.25).sum()
+        loss.backward()
+        return loss
+    assert float(opt.step(closure, max_norm=1.0)) == 75.0
+    assert_norm(opt.grad_norm, 0.25 * math.sqrt(300), 2.0)
 
 
 def test_step_missing_gradients_and_refusals():
