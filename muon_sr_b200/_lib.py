@@ -161,6 +161,17 @@ def load():
     return _lib
 
 
+def native():
+    """The binding of the gradient norm (``csrc/binding.cpp``), built with the library."""
+    load()  # the library it calls, with the environment's knobs applied
+    try:
+        from . import _native
+    except ImportError as e:
+        raise RuntimeError("muon_sr_b200: the binding _native.so is missing or was built for another torch; build it "
+                           f"with `python -m muon_sr_b200.build` ({e})") from e
+    return _native
+
+
 # Process-wide debug knobs read once, when the library loads: MSR_SR_NOISE selects the
 # stochastic-rounding noise ("none" = round to nearest, the parity mode), MSR_GEMM_PAIRS=0
 # the single-SM GEMM tiles. Both give the same API; see msr_set_sr_noise / msr_set_gemm_pairs.

@@ -1,4 +1,5 @@
-"""Build the engine's C-ABI shared library, ``muon_sr_b200/libmuon_sr_b200.so``, with nvcc.
+"""Build the engine's C-ABI shared library, ``muon_sr_b200/libmuon_sr_b200.so``, with nvcc, and
+the Python binding of the gradient norm, ``muon_sr_b200/_native.so``, against the installed torch.
 
     python -m muon_sr_b200.build [--verbose-ptxas] [--force]
 
@@ -14,11 +15,13 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libmuon_sr_b200.so")
+BINDING = os.path.join(PKG, "_native.so")
 INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -43,7 +46,8 @@ def _deps_mtime():
 
 
 def build(force: bool = False, verbose_ptxas: bool = False) -> str:
-    if not force and os.path.exists(LIB) and os.path.getmtime(LIB) >= _deps_mtime():
+    built = [os.path.getmtime(f) for f in (LIB, BINDING) if os.path.exists(f)]
+    if not force and len(built) == 2 and min(built) >= _deps_mtime():
         return LIB
     os.makedirs(BUILD, exist_ok=True)
     cc = nvcc()
@@ -61,7 +65,9 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
         return obj, r.stderr
 
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        binding = ex.submit(_compile_binding, os.path.join(BUILD, "binding.o"))
         results = list(ex.map(compile_one, sources()))
+        binding.result()
     if verbose_ptxas:
         for obj, err in results:
             sys.stderr.write(f"== {os.path.basename(obj)}\n{err}")
@@ -71,7 +77,32 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"nvcc link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    _link_binding(os.path.join(BUILD, "binding.o"))
     return LIB
+
+
+def _run(cmd, what):
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{what} failed:\n{r.stdout}\n{r.stderr}")
+
+
+def _compile_binding(obj):
+    import torch
+    root = os.path.join(os.path.dirname(torch.__file__), "include")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
+    dirs = [root, os.path.join(root, "torch", "csrc", "api", "include"), cuda, sysconfig.get_paths()["include"]]
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *[f"-isystem{d}" for d in dirs], "-c", os.path.join(CSRC, "binding.cpp"), "-o", obj], "g++ on binding.cpp")
+
+
+def _link_binding(obj):
+    import torch
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = BINDING + ".tmp"
+    _run(["g++", "-shared", "-o", tmp, obj, f"-L{PKG}", "-lmuon_sr_b200", f"-L{libs}", "-ltorch_python", "-ltorch_cpu",
+          "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"], "linking the binding")
+    os.replace(tmp, BINDING)
 
 
 def main():

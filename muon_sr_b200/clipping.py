@@ -57,10 +57,15 @@ def get_total_norm(tensors, norm_type=2.0, error_if_nonfinite=False, *, per_tens
     if not tensors:
         total = torch.zeros(())
         return (total, torch.zeros(0)) if per_tensor else total
-    norm = K.grad_norm(K.GradTable(tensors), norm_type, per_tensor=per_tensor)
+    plain = K.plain_grad_norm(tensors, norm_type, 1.0, math.inf, per_tensor)
+    if plain is not None:
+        _, total, each = plain
+    else:
+        norm = K.grad_norm(K.GradTable(tensors), norm_type, per_tensor=per_tensor)
+        total, each = norm.norm, norm.each
     if error_if_nonfinite:
-        _refuse_nonfinite(norm.norm, norm_type)
-    return (norm.norm, norm.each) if per_tensor else norm.norm
+        _refuse_nonfinite(total, norm_type)
+    return (total, each) if per_tensor else total
 
 
 def _norm_over_ranks(table, norm_type, grad_scale, max_norm, shard):
@@ -93,13 +98,18 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     whose gradients share memory are refused."""
     norm_type = _norm_type(norm_type)
     max_norm, grad_scale = _bounds(max_norm, grad_scale)
-    table = _gradients([parameters] if isinstance(parameters, torch.Tensor) else parameters, shard)
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    whole = shard is None and not error_if_nonfinite
+    if whole and not staging.active() and \
+            (norm := K.plain_grad_clip_(parameters, norm_type, grad_scale, max_norm)) is not None:
+        return norm
+    table = _gradients(parameters, shard)
     if table is None:
         return torch.zeros(())
     if table.dense is not table.grads and any(st == 0 and n > 1 for g in table.grads
                                               for st, n in zip(g.stride(), g.shape)):
         raise ValueError("gradients must not be expanded tensors: their elements share memory")
-    if shard is None and not error_if_nonfinite:
+    if whole:
         return K.grad_clip_(table, norm_type, grad_scale, max_norm).norm
     norm = _norm_over_ranks(table, norm_type, grad_scale, max_norm, shard)
     if error_if_nonfinite:
@@ -111,7 +121,6 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
 def _gradients(parameters, shard):
     """The ``GradTable`` of the parameters that have a gradient, each once (with a sharder: those
     of them that this rank owns), or None where there is nothing to launch."""
-    parameters = list(parameters)
     grads = [g for p in parameters if (g := p.grad) is not None]
     if shard is not None or staging.active() or len(set(map(id, grads))) < len(grads):
         params = list({id(p): p for p in parameters if p.grad is not None}.values())
@@ -137,9 +146,16 @@ def clipped_step(optimizer, max_norm, grad_scale):
     shard = getattr(optimizer, "_shard", None)
     if shard is not None:
         shard._ensure(optimizer)
-    table = _gradients([p for g in optimizer.param_groups for p in g["params"]], shard)
-    if table is None:
-        return contextlib.nullcontext()
-    norm = _norm_over_ranks(table, 2.0, grad_scale, max_norm, shard)
+    params = [p for g in optimizer.param_groups for p in g["params"]]
+    plain = None
+    if shard is None and not staging.active():
+        plain = K.plain_grad_norm(params, 2.0, grad_scale, max_norm, of_grads=True)
+    if plain is not None:
+        norm = K.GradNorm(None, state=plain[0])
+    else:
+        table = _gradients(params, shard)
+        if table is None:
+            return contextlib.nullcontext()
+        norm = _norm_over_ranks(table, 2.0, grad_scale, max_norm, shard)
     optimizer.grad_norm = norm.norm
     return K.gradient_factor(norm.factor)

@@ -440,8 +440,10 @@ class GradNorm:
 
     __slots__ = ("state", "each")
 
-    def __init__(self, device, count=None):
-        self.state = torch.empty(ctypes.sizeof(_lib.ClipState) // 4, dtype=torch.float32, device=device)
+    def __init__(self, device, count=None, state=None):
+        self.state = state
+        if state is None:
+            self.state = torch.empty(ctypes.sizeof(_lib.ClipState) // 4, dtype=torch.float32, device=device)
         self.each = None if count is None else torch.empty(count, dtype=torch.float32, device=device)
 
     @property
@@ -488,6 +490,20 @@ def grad_norm(table: GradTable, norm_type: float = 2.0, scale: float = 1.0, max_
     _launch(index, "msr_grad_norm", table.address(), count, NORM_TYPES[norm_type], scale, max_norm,
             out.state.data_ptr(), None if out.each is None else out.each.data_ptr(), ws.data_ptr(), nbytes)
     return out
+
+
+def plain_grad_norm(tensors, norm_type: float, scale: float, max_norm: float, per_tensor=False, of_grads=False):
+    """``grad_norm`` of a list of plain tensors (with ``of_grads``, of parameters' gradients) by
+    the native binding, as ``(state, norm, each)``; None where it does not serve them -- another
+    layout, a repetition, nothing at all, a step being recorded -- and nothing was done."""
+    if _recorder() is not None:
+        return None
+    return _lib.native().grad_norm(tensors, NORM_TYPES[norm_type], scale, max_norm, per_tensor, of_grads)
+
+
+def plain_grad_clip_(parameters, norm_type: float, scale: float, max_norm: float):
+    """``grad_clip_`` of the gradients of a list of parameters, likewise: the norm or None."""
+    return _lib.native().grad_clip(parameters, NORM_TYPES[norm_type], scale, max_norm)
 
 
 def grad_factor(norm: GradNorm, norm_type: float, scale: float, max_norm: float) -> None:

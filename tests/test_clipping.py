@@ -45,6 +45,16 @@ def test_refusals():
         opt.step(grad_scale=0.5)
 
 
+def test_binding_serves_cuda_tensors_only():
+    p = _param()
+    for args in ([p.grad], [], [None], (p.grad,)):
+        assert K.plain_grad_norm(args, 2.0, 1.0, 1.0) is None
+    for args in ([p], [], [None], [torch.nn.Parameter(torch.zeros(3))], (p,)):
+        assert K.plain_grad_clip_(args, 2.0, 1.0, 1.0) is None
+    with pytest.raises(TypeError):
+        _lib.native().grad_clip()
+
+
 def test_nothing_to_clip():
     assert float(get_total_norm([])) == 0.0
     total, each = get_total_norm([], per_tensor=True)

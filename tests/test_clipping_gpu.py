@@ -440,6 +440,37 @@ def test_clip_lists_and_refusals():
         clip_grad_norm_([s], 1.0)
 
 
+def test_binding_and_tables_agree(monkeypatch):
+    """Plain gradients go through the native binding, anything else through tables built in
+    Python: the same bits, and the binding serves what it says and nothing else."""
+    _, grads = make([70001, 9, 300, 8192], torch.bfloat16)
+    params = params_of(grads)
+    assert K.plain_grad_norm(grads, 2.0, 1.0, 1.0) is not None
+    assert K.plain_grad_norm(grads + grads[:1], 2.0, 1.0, 1.0) is not None      # a repetition counts twice
+    total2 = get_total_norm(grads + grads)
+    assert_norm(total2, norm64(grads + grads, 2.0)[0], 2.0)
+    other = torch.nn.Parameter(torch.empty_like(grads[0]))
+    other.grad = grads[0].view(-1)[:]
+    nongrad = torch.nn.Parameter(torch.zeros(2, device=DEV))
+    strided = torch.zeros(6, 8, device=DEV)[:, :4]
+    for refused in ([], [nongrad], params + params[:1], [params[0], other], [strided.requires_grad_() * 2], [3], [None]):
+        assert K.plain_grad_clip_(refused, 2.0, 1.0, 1.0) is None
+    for refused in ([], (grads[0],), [strided], [grads[0], torch.zeros(3)], [grads[0].double()], [None]):
+        assert K.plain_grad_norm(refused, 2.0, 1.0, 1.0) is None
+    results = []
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(K, "plain_grad_norm", lambda *a, **k: None)
+            monkeypatch.setattr(K, "plain_grad_clip_", lambda *a, **k: None)
+        ps = params_of([g.clone() for g in grads])
+        total, each = get_total_norm([p.grad for p in ps], per_tensor=True)
+        opt = TritonAdamW(ps)
+        opt.step(max_norm=0.5, grad_scale=2.0)
+        norm = clip_grad_norm_(ps, 0.5, grad_scale=2.0)
+        results.append([total, each, opt.grad_norm, norm] + [p.grad for p in ps] + [opt.state[p]["ema"] for p in ps])
+    assert all(same_bits(a, b) for a, b in zip(*results))
+
+
 def test_two_calls_on_two_streams():
     streams = [torch.cuda.Stream() for _ in range(2)]
     sets = [make([3000001 + k, 70], torch.bfloat16, seed=k)[1] for k in range(2)]
