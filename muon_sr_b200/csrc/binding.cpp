@@ -22,6 +22,7 @@ namespace {
 
 struct Gradients {
   std::vector<msr_grad_entry> entries;
+  std::vector<c10::TensorImpl*> tensors;  // alive as long as the list they came from
   int device = -1;
 };
 
@@ -40,6 +41,7 @@ bool collect(PyObject* list, bool of_grads, Gradients& out) {
   if (!PyList_CheckExact(list)) return false;
   const Py_ssize_t n = PyList_GET_SIZE(list);
   out.entries.reserve(n);
+  out.tensors.reserve(n);
   for (Py_ssize_t i = 0; i < n; ++i) {
     PyObject* item = PyList_GET_ITEM(list, i);
     if (!THPVariable_Check(item)) return false;
@@ -57,6 +59,7 @@ bool collect(PyObject* list, bool of_grads, Gradients& out) {
     const int device = g.get_device();
     if (code < 0 || (out.device >= 0 && device != out.device)) return false;
     out.device = device;
+    out.tensors.push_back(g.unsafeGetTensorImpl());
     out.entries.push_back(msr_grad_entry{g.numel() ? g.data_ptr() : nullptr, g.numel(), code, 0});
   }
   return !out.entries.empty();
@@ -132,6 +135,8 @@ PyObject* grad_clip(PyObject*, PyObject* args) {
   check(msr_grad_clip(g.entries.data(), static_cast<int>(g.entries.size()), norm, scale, max_norm, call.st(),
                       call.workspace.data_ptr(), call.bytes, call.stream),
         "msr_grad_clip");
+  for (c10::TensorImpl* t : g.tensors)  // autograd sees the write, as after any in-place operation
+    if (!t->is_inference()) t->bump_version();
   return THPVariable_Wrap(call.norm());
   END_HANDLE_TH_ERRORS
 }

@@ -532,6 +532,9 @@ def grad_clip_(table: GradTable, norm_type: float, scale: float, max_norm: float
 
 
 def _copy_back(table):
+    """After a scaling: autograd sees the write, as after any in-place operation, and gradients
+    that were scaled in a copy get it back."""
+    torch.autograd.graph.increment_version([d for d in table.dense if not d.is_inference()])
     if table.dense is not table.grads:
         with torch.no_grad():
             for g, d in zip(table.grads, table.dense):

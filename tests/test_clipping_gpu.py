@@ -471,6 +471,25 @@ def test_binding_and_tables_agree(monkeypatch):
     assert all(same_bits(a, b) for a, b in zip(*results))
 
 
+@pytest.mark.parametrize("native", [True, False])
+def test_clip_counts_as_an_in_place_write(native, monkeypatch):
+    """A graph that saved a gradient (double backward) notices that it was clipped."""
+    if not native:
+        monkeypatch.setattr(K, "plain_grad_clip_", lambda *a, **k: None)
+    p = torch.nn.Parameter(torch.ones(40, device=DEV))
+    (p ** 3).sum().backward()
+    p.grad.requires_grad_()
+    loss = (p.grad ** 2).sum()                               # saves p.grad
+    clip_grad_norm_(p, 1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    with torch.inference_mode():
+        q = torch.nn.Parameter(torch.ones(40, device=DEV))
+        q.grad = torch.ones(40, device=DEV)
+        assert_norm(clip_grad_norm_(q, 1.0), math.sqrt(40), 2.0)
+    assert_scaled(q.grad, torch.ones(40, device=DEV), 1 / (math.sqrt(40) + 1e-6))
+
+
 def test_two_calls_on_two_streams():
     streams = [torch.cuda.Stream() for _ in range(2)]
     sets = [make([3000001 + k, 70], torch.bfloat16, seed=k)[1] for k in range(2)]
