@@ -67,7 +67,6 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         binding = ex.submit(_compile_binding, os.path.join(BUILD, "binding.o"))
         results = list(ex.map(compile_one, sources()))
-        binding.result()
     if verbose_ptxas:
         for obj, err in results:
             sys.stderr.write(f"== {os.path.basename(obj)}\n{err}")
@@ -77,6 +76,7 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"nvcc link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    binding.result()  # after the library, which does not need it
     _link_binding(os.path.join(BUILD, "binding.o"))
     return LIB
 

@@ -511,10 +511,11 @@ def test_clip_captured_in_two_graphs():
     """Two graphs captured on one stream replay on two others at once, over new gradients."""
     sets = [make([2000003, 70], torch.bfloat16, seed=k)[1] for k in range(2)]
     clip_grad_norm_(params_of(sets[0]), math.inf)
-    graphs, norms = [], []
+    graphs, norms, totals = [], [], []
     for grads in sets:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
+            totals.append(get_total_norm(grads, per_tensor=True))
             norms.append(clip_grad_norm_(params_of(grads), 0.5))
         graphs.append(g)
     streams = [torch.cuda.Stream() for _ in graphs]
@@ -530,7 +531,10 @@ def test_clip_captured_in_two_graphs():
             with torch.cuda.stream(s):
                 g.replay()
         torch.cuda.synchronize()
-        for norm, want, grads, old in zip(norms, wants, sets, before):
+        for (total, each), norm, want, grads, old in zip(totals, norms, wants, sets, before):
+            assert_norm(total, want, 2.0)
+            for e, b in zip(each.tolist(), norm64(old, 2.0)[1]):
+                assert_norm(e, b, 2.0)
             assert_norm(norm, want, 2.0)
             for g, b in zip(grads, old):
                 assert_scaled(g, b, 0.5 / (want + 1e-6))
