@@ -67,7 +67,7 @@ class TritonAdamW(Optimizer):
         centralization (float): gradient centralization strength (default: 0)
 
     ``step(max_norm=, grad_scale=)`` clips the gradients by their global norm as it reads them
-    (see ``clipping``).
+    (see ``clipping``); with centralization the norm is that of the gradients before it.
     """
 
     grad_norm = None  # the last step's gradient norm, where it clipped
