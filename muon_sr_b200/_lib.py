@@ -5,6 +5,7 @@ is no fallback: if the library is missing or cannot load, every optimizer step r
 """
 import ctypes
 import os
+import sysconfig
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -161,15 +162,31 @@ def load():
     return _lib
 
 
+def built_for() -> str:
+    """What the binding is built against: torch, its C++ ABI and the interpreter's."""
+    import torch
+    return f"torch {torch.__version__} abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)} {sysconfig.get_config_var('SOABI')}"
+
+
+_native_module = None
+
+
 def native():
     """The binding of the gradient norm (``csrc/binding.cpp``), built with the library."""
-    load()  # the library it calls, with the environment's knobs applied
-    try:
-        from . import _native
-    except ImportError as e:
-        raise RuntimeError("muon_sr_b200: the binding _native.so is missing or was built for another torch; build it "
-                           f"with `python -m muon_sr_b200.build` ({e})") from e
-    return _native
+    global _native_module
+    if _native_module is None:
+        load()  # the library it calls, with the environment's knobs applied
+        try:
+            from . import _native
+        except ImportError as e:
+            raise RuntimeError("muon_sr_b200: the binding _native.so is missing or was built for another torch; build "
+                               f"it with `python -m muon_sr_b200.build` ({e})") from e
+        # (one built for another torch may load all the same and read tensors at that one's offsets)
+        if getattr(_native, "built_for", None) != built_for():
+            raise RuntimeError(f"muon_sr_b200: the binding _native.so was built for {getattr(_native, 'built_for', None)}"
+                               f", this is {built_for()}; build it with `python -m muon_sr_b200.build`")
+        _native_module = _native
+    return _native_module
 
 
 # Process-wide debug knobs read once, when the library loads: MSR_SR_NOISE selects the

@@ -3,6 +3,7 @@ the Python binding of the gradient norm, ``muon_sr_b200/_native.so``, against th
 
     python -m muon_sr_b200.build [--verbose-ptxas] [--force]
 
+builds what is older than its sources, and the binding again under another torch or interpreter.
 Every CUDA source under ``csrc/`` is compiled for sm_100a only
 (``-gencode arch=compute_100a,code=sm_100a``) and linked with the static CUDA runtime into
 one in-tree shared object that the Python layer loads with ctypes. The elementwise and
@@ -17,11 +18,15 @@ import subprocess
 import sys
 import sysconfig
 
+from ._lib import built_for
+
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libmuon_sr_b200.so")
 BINDING = os.path.join(PKG, "_native.so")
+BINDING_OBJ = os.path.join(BUILD, "binding.o")
+BINDING_FOR = os.path.join(BUILD, "binding.for")  # what the binding was built against
 INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -45,11 +50,27 @@ def _deps_mtime():
     return max(os.path.getmtime(f) for f in files)
 
 
+def _current(path):
+    return os.path.exists(path) and os.path.getmtime(path) >= _deps_mtime()
+
+
+def _binding_current():
+    """Whether the binding is newer than its sources and built against this torch: it holds
+    torch's inline accessors and the interpreter's ABI, which file times say nothing of."""
+    if not _current(BINDING) or not os.path.exists(BINDING_FOR):
+        return False
+    with open(BINDING_FOR) as f:
+        return f.read() == built_for()
+
+
 def build(force: bool = False, verbose_ptxas: bool = False) -> str:
-    built = [os.path.getmtime(f) for f in (LIB, BINDING) if os.path.exists(f)]
-    if not force and len(built) == 2 and min(built) >= _deps_mtime():
+    library = force or not _current(LIB)
+    if not library and _binding_current():
         return LIB
     os.makedirs(BUILD, exist_ok=True)
+    if not library:
+        _build_binding()
+        return LIB
     cc = nvcc()
 
     def compile_one(src):
@@ -65,7 +86,7 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
         return obj, r.stderr
 
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
-        binding = ex.submit(_compile_binding, os.path.join(BUILD, "binding.o"))
+        binding = ex.submit(_compile_binding)
         results = list(ex.map(compile_one, sources()))
     if verbose_ptxas:
         for obj, err in results:
@@ -77,7 +98,7 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
         raise RuntimeError(f"nvcc link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
     binding.result()  # after the library, which does not need it
-    _link_binding(os.path.join(BUILD, "binding.o"))
+    _link_binding()
     return LIB
 
 
@@ -87,22 +108,30 @@ def _run(cmd, what):
         raise RuntimeError(f"{what} failed:\n{r.stdout}\n{r.stderr}")
 
 
-def _compile_binding(obj):
+def _build_binding():
+    _compile_binding()
+    _link_binding()
+
+
+def _compile_binding():
     import torch
     root = os.path.join(os.path.dirname(torch.__file__), "include")
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
     dirs = [root, os.path.join(root, "torch", "csrc", "api", "include"), cuda, sysconfig.get_paths()["include"]]
     _run(["g++", "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-          *[f"-isystem{d}" for d in dirs], "-c", os.path.join(CSRC, "binding.cpp"), "-o", obj], "g++ on binding.cpp")
+          f'-DMSR_BUILT_FOR="{built_for()}"', *[f"-isystem{d}" for d in dirs], "-c", os.path.join(CSRC, "binding.cpp"),
+          "-o", BINDING_OBJ], "g++ on binding.cpp")
 
 
-def _link_binding(obj):
+def _link_binding():
     import torch
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     tmp = BINDING + ".tmp"
-    _run(["g++", "-shared", "-o", tmp, obj, f"-L{PKG}", "-lmuon_sr_b200", f"-L{libs}", "-ltorch_python", "-ltorch_cpu",
+    _run(["g++", "-shared", "-o", tmp, BINDING_OBJ, f"-L{PKG}", "-lmuon_sr_b200", f"-L{libs}", "-ltorch_python", "-ltorch_cpu",
           "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"], "linking the binding")
     os.replace(tmp, BINDING)
+    with open(BINDING_FOR, "w") as f:
+        f.write(built_for())
 
 
 def main():
