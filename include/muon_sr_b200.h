@@ -316,7 +316,9 @@ int msr_grad_clip(const msr_grad_entry* entries, int count, int norm, double sca
 /* The updates above with every gradient read as g * grad_factor[0], an fp32 scalar in device
  * memory (state->factor of msr_grad_norm): the product is taken in fp32 and is not rounded to
  * bf16, and the gradients themselves stay. Everything else -- noise, order of the operations,
- * records -- is that of the call without the suffix, and grad_factor[0] = 1 gives its bits. */
+ * records -- is that of the call without the suffix, and grad_factor[0] = 1 gives its bits.
+ * msr_adamw8bit_scaled with a grad_factor[0] that is not finite changes nothing at all: its rule for
+ * non-finite gradients, resetting their moments, would reset every element's. */
 int msr_muon_prepare_scaled(const msr_prepare_entry* entries, int count, float beta, float one_minus_beta,
                             int nesterov, const float* grad_factor, msr_stream_t stream);
 int msr_adamw_sr_scaled(const msr_adamw_entry* entries, int count, const msr_adamw_hparams* hp,

@@ -12,7 +12,8 @@
 The first two take the arguments of their namesakes in ``torch.nn.utils``. Sums are kept in
 double and norms returned in fp32, whatever the gradients' type, on the device: nothing here
 waits for the GPU unless ``error_if_nonfinite`` asks for it. A step whose norm is not finite
-does what scaling by such a factor would: look at ``grad_norm`` where that can happen.
+does what scaling by such a factor would -- except that the 8-bit AdamW step by a NaN norm leaves
+weights and moments as they were: look at ``grad_norm`` where that can happen.
 """
 import contextlib
 import math

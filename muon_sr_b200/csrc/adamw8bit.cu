@@ -136,6 +136,11 @@ __global__ __launch_bounds__(Q_THREADS, 4) void adamw8bit_kernel(const __grid_co
   constexpr int EPT = BS > 2048 ? 16 : 8;
   constexpr int TILE = Q_THREADS * EPT;
   constexpr int G = BS / EPT;  // threads per quantisation block
+  const float gs = SCALED ? *a.gscale : 1.f;
+  // A factor that is not finite (one NaN among all gradients) would make every gradient so, and the
+  // rule below, which resets the moments of such an element, would empty the whole optimizer:
+  // the launch leaves everything as it is instead.
+  if (SCALED && !finite_f(gs)) return;
   extern __shared__ __align__(16) uint8_t dsm[];
   float* q1 = reinterpret_cast<float*>(dsm);
   float* q2 = q1 + 256;
@@ -157,7 +162,6 @@ __global__ __launch_bounds__(Q_THREADS, 4) void adamw8bit_kernel(const __grid_co
   const float* t_pos2 = t_pos1 + 512;
   __syncthreads();
   const msr_adamw8bit_hparams hp = a.hp;
-  const float gs = SCALED ? *a.gscale : 1.f;
   const int64_t total = a.prefix[a.count];
   int ei = blockIdx.x < total ? find_entry<Q_MAXE>(a.prefix, a.count, blockIdx.x) : 0;
   for (int64_t tile = blockIdx.x; tile < total; tile += gridDim.x) {

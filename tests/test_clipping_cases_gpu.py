@@ -1,0 +1,95 @@
+"""Clipping on the GPU where its callers' data goes wrong: non-finite norms, gradients that
+share memory."""
+import math
+
+import pytest
+import torch
+
+from muon_sr_b200 import TritonAdamW8bit
+from muon_sr_b200 import kernels as K
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def raw(t):
+    return t.detach().contiguous().view(-1).view(torch.uint8)
+
+
+def same_bits(a, b):
+    return torch.equal(raw(a), raw(b))
+
+
+# ---- the 8-bit step under a non-finite norm ---------------------------------------------
+SIZES = [5000, 300, 8192, 4097]  # block tails, and one below min_8bit_size (bf16 moments)
+
+
+def eight_bit(block_size):
+    gen = torch.Generator().manual_seed(3)
+    params = [torch.nn.Parameter((torch.randn(n, generator=gen) * 0.02).to(torch.bfloat16).to(DEV)) for n in SIZES]
+    return params, TritonAdamW8bit(params, lr=1e-3, weight_decay=0.01, min_8bit_size=512, block_size=block_size)
+
+
+def fill(params, seed):
+    gen = torch.Generator().manual_seed(seed)
+    for p in params:
+        p.grad = (torch.randn(p.shape, generator=gen) * 1e-2).to(torch.bfloat16).to(DEV)
+
+
+def tensors_of(params, opt):
+    return [t for p in params for t in (p, *(v for _, v in sorted(opt.state[p].items()) if torch.is_tensor(v)))]
+
+
+@pytest.mark.parametrize("lookup", [True, False])
+@pytest.mark.parametrize("block_size", [64, 256, 4096])
+def test_8bit_step_by_a_nan_norm_leaves_everything(block_size, lookup, monkeypatch):
+    """One NaN makes the norm and the factor NaN: no parameter's moments may be lost to it."""
+    if not lookup:
+        monkeypatch.setattr(K, "quant_tables", lambda *a: None)
+    params, opt = eight_bit(block_size)
+    for step in range(2):
+        fill(params, step)
+        opt.step(max_norm=1.0)
+    before = [t.detach().clone() for t in tensors_of(params, opt)]
+    weights = [p.detach().clone() for p in params]
+    fill(params, 2)
+    params[0].grad[77] = math.nan
+    opt.step(max_norm=1.0)
+    assert math.isnan(float(opt.grad_norm))
+    for i, (a, b) in enumerate(zip(tensors_of(params, opt), before)):
+        assert same_bits(a, b), i
+    fill(params, 3)                                           # and training goes on
+    opt.step(max_norm=1.0)
+    assert math.isfinite(float(opt.grad_norm))
+    assert not any(same_bits(p, w) for p, w in zip(params, weights))
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_8bit_step_with_a_finite_factor_keeps_the_rule_of_each_element(bad):
+    """max_norm = inf clips nothing, so the factor stays 1 whatever the norm, and a non-finite
+    gradient touches its own element alone, as in a step without clipping."""
+    (pa, oa), (pb, ob) = eight_bit(256), eight_bit(256)
+    for step in range(2):
+        for ps in (pa, pb):
+            fill(ps, step)
+            ps[2].grad[4000] = bad
+        oa.step()
+        ob.step(max_norm=math.inf)
+        assert not math.isfinite(float(ob.grad_norm))
+        assert all(same_bits(a, b) for a, b in zip(tensors_of(pa, oa), tensors_of(pb, ob)))
+
+
+def test_8bit_step_by_an_infinite_norm_is_that_of_scaled_gradients():
+    """Infinity gives a factor of 0: gradients of 0 and, where they were infinite, NaN."""
+    (pa, oa), (pb, ob) = eight_bit(256), eight_bit(256)
+    for ps, o in ((pa, oa), (pb, ob)):
+        fill(ps, 0)
+        o.step()
+        fill(ps, 1)
+        ps[3].grad[5] = -math.inf
+    for p in pa:
+        p.grad.mul_(0.0)
+    oa.step()
+    ob.step(max_norm=1.0)
+    assert float(ob.grad_norm) == math.inf
+    assert all(same_bits(a, b) for a, b in zip(tensors_of(pa, oa), tensors_of(pb, ob)))
