@@ -17,7 +17,9 @@ weights and moments as they were: look at ``grad_norm`` where that can happen.
 """
 import contextlib
 import math
+import operator
 
+import numpy as np
 import torch
 
 from . import kernels as K
@@ -107,9 +109,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     table = _gradients(parameters, shard)
     if table is None:
         return torch.zeros(())
-    if table.dense is not table.grads and any(st == 0 and n > 1 for g in table.grads
-                                              for st, n in zip(g.stride(), g.shape)):
-        raise ValueError("gradients must not be expanded tensors: their elements share memory")
+    if table.dense is not table.grads:
+        _refuse_shared(table)
     if whole:
         return K.grad_clip_(table, norm_type, grad_scale, max_norm).norm
     norm = _norm_over_ranks(table, norm_type, grad_scale, max_norm, shard)
@@ -117,6 +118,44 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         _refuse_nonfinite(norm.norm, norm_type)
     K.grad_scale_(table, norm)
     return norm.norm
+
+
+class _Place:
+    """The elements of a CUDA tensor as an array interface: numpy solves for common elements from
+    address, shape and strides alone."""
+
+    def __init__(self, t):
+        size = t.element_size()
+        self.__array_interface__ = dict(version=3, typestr=f"|V{size}", shape=tuple(t.shape),
+                                        strides=tuple(st * size for st in t.stride()), data=(t.data_ptr(), True))
+
+
+_SHARES_WORK = 1_000_000  # steps of numpy's search, far above what views of matrices take
+
+
+def _refuse_shared(table):
+    """Raise where a gradient that goes through a copy is expanded or shares elements with
+    another: the copies lie apart, so the check of the scaling itself would not see it."""
+    if any(st == 0 and n > 1 for g in table.grads for st, n in zip(g.stride(), g.shape)):
+        raise ValueError("gradients must not be expanded tensors: their elements share memory")
+    spans = []
+    for g, d in zip(table.grads, table.dense):
+        if g.numel():
+            last = sum(st * (n - 1) for st, n in zip(g.stride(), g.shape))
+            spans.append((g.data_ptr(), g.data_ptr() + (last + 1) * g.element_size(), g is d, np.asarray(_Place(g))))
+    spans.sort(key=operator.itemgetter(0))
+    reach = []  # those before that end behind the present one's start
+    for span in spans:
+        reach = [s for s in reach if s[1] > span[0]]
+        for other in reach:
+            if not (span[2] and other[2]):  # (two dense ones are checked with their launch)
+                try:
+                    shared = np.shares_memory(span[3], other[3], max_work=_SHARES_WORK)
+                except np.exceptions.TooHardError:
+                    shared = True
+                if shared:
+                    raise RuntimeError("two gradients overlap in memory")
+        reach.append(span)
 
 
 def _gradients(parameters, shard):

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from muon_sr_b200 import TritonAdamW8bit
+from muon_sr_b200 import TritonAdamW8bit, clip_grad_norm_
 from muon_sr_b200 import kernels as K
 
 pytestmark = pytest.mark.gpu
@@ -93,3 +93,53 @@ def test_8bit_step_by_an_infinite_norm_is_that_of_scaled_gradients():
     ob.step(max_norm=1.0)
     assert float(ob.grad_norm) == math.inf
     assert all(same_bits(a, b) for a, b in zip(tensors_of(pa, oa), tensors_of(pb, ob)))
+
+# ---- gradients that share memory ---------------------------------------------------------
+def clip(grads, max_norm=0.5):
+    params = []
+    for g in grads:
+        p = torch.nn.Parameter(torch.empty(g.shape, dtype=g.dtype, device=DEV))
+        p.grad = g
+        params.append(p)
+    return clip_grad_norm_(params, max_norm)
+
+
+@pytest.mark.parametrize("views", [
+    lambda x: [x[:, 2:30], x[:, 2:30]],                      # one non-dense view twice
+    lambda x: [x[:, 2:30], x[:, 29:40]],                     # a column in common
+    lambda x: [x[::2], x[4:9]],                              # rows in common, one view dense
+    lambda x: [x, x[:, 5]],
+    lambda x: [x[:, ::3], x[:, ::2].t()],
+    lambda x: [x[:10, :7], x[20:, 9:], x[9:21, 6:10]],       # the third meets both
+])
+def test_strided_gradients_that_share_memory_are_refused(views):
+    x = torch.randn(40, 64, device=DEV).to(torch.bfloat16)
+    before = x.clone()
+    with pytest.raises(RuntimeError, match="overlap in memory"):
+        clip(views(x))
+    assert same_bits(x, before)
+
+
+@pytest.mark.parametrize("views", [
+    lambda x: [x[:, 0::2], x[:, 1::2]],                      # interleaved, nothing in common
+    lambda x: [x[:, :30], x[:, 30:].t()],
+    lambda x: [x[::2], x[1::2, 3:], x[1::2, :3]],
+    lambda x: [x[:, i] for i in range(64)],
+    lambda x: [x[:, 5][:0], x[:, 5], x[:, 5][:0]],           # empty views share nothing
+])
+def test_strided_gradients_side_by_side_are_clipped(views):
+    x = torch.randn(40, 64, device=DEV).to(torch.bfloat16)
+    before = x.clone()
+    grads = views(x)
+    want = math.sqrt(sum(float((g.double() ** 2).sum()) for g in grads))
+    # norm: 33 roundings of fp32 at most on the power, halved by the root, and one more
+    assert abs(float(clip(grads, want / 4)) - want) <= 34 * 2.0 ** -24 * want
+    factor = (want / 4) / (want + 1e-6)
+    inside = torch.zeros_like(x, dtype=torch.bool)
+    for g in views(inside):
+        g.fill_(True)
+    scaled = before.double() * factor
+    # half a bf16 step, the factor's error and a product's (34 + 1 + 1 roundings of fp32)
+    tol = scaled.abs() * (2.0 ** -8 + 37 * 2.0 ** -24) + 2.0 ** -134
+    assert bool(((x.double() - scaled).abs() <= tol)[inside].all())
+    assert torch.equal(x[~inside], before[~inside])
