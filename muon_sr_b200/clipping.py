@@ -170,7 +170,13 @@ def _gradients(parameters, shard):
         grads = [p.grad for p in params]
     if not grads and shard is None:
         return None
-    return K.GradTable(grads, None if grads else torch.cuda.current_device())
+    return K.GradTable(grads, None if grads else _device_of(parameters))
+
+
+def _device_of(parameters):
+    """The device on which a rank that owns none of the gradients joins the others' sum."""
+    first = min(parameters, key=lambda p: p.grad is None, default=None)
+    return torch.cuda.current_device() if first is None else first.get_device()
 
 
 def clipped_step(optimizer, max_norm, grad_scale):

@@ -415,6 +415,8 @@ class GradTable:
     def __init__(self, grads, device=None):
         self.grads = self.dense = grads
         if not grads:
+            if device < 0:
+                raise ValueError("gradients must be CUDA tensors (muon_sr_b200 has no CPU path)")
             self.words, self.index = array.array("q"), device
             return
         self.index = grads[0].get_device()

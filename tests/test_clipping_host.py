@@ -1,0 +1,40 @@
+"""The host's side of clipping, without a GPU: where a rank without gradients puts its state."""
+import types
+
+import pytest
+import torch
+
+from muon_sr_b200 import clipping
+from muon_sr_b200 import kernels as K
+
+
+class OnDevice:
+    """A parameter of CUDA device `index` as far as the tables look at one."""
+
+    def __init__(self, index, grad=True):
+        self.index, self.grad = index, grad or None
+
+    def get_device(self):
+        return self.index
+
+
+@pytest.mark.parametrize("params,want", [
+    ([OnDevice(1), OnDevice(1)], 1),
+    ([OnDevice(0, grad=False), OnDevice(1)], 1),   # those with a gradient come first
+    ([OnDevice(1, grad=False)], 1),
+    ([], 3),                                       # nothing says where: the current device
+])
+def test_rank_without_gradients_uses_the_parameters_device(params, want, monkeypatch):
+    made = []
+    monkeypatch.setattr(K, "GradTable", lambda grads, device=None: made.append((grads, device)))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    clipping._gradients(params, types.SimpleNamespace(owned=lambda ps: []))
+    assert made == [([], want)]
+
+
+def test_rank_without_gradients_refuses_cpu_parameters():
+    """As the ranks that hold the gradients do, so that none waits for another."""
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.ones(3)
+    with pytest.raises(ValueError, match="no CPU path"):
+        clipping._gradients([p], types.SimpleNamespace(owned=lambda ps: []))
