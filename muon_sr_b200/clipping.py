@@ -48,13 +48,14 @@ def _refuse_nonfinite(norm, norm_type):
                            "clipped. Pass error_if_nonfinite=False to clip with the non-finite norm anyway.")
 
 
-def get_total_norm(tensors, norm_type=2.0, error_if_nonfinite=False, *, per_tensor=False):
+def get_total_norm(tensors, norm_type=2.0, error_if_nonfinite=False, foreach=None, *, per_tensor=False):
     """The norm of ``tensors`` (bf16, fp16 or fp32 CUDA tensors on one device, mixed at will) as
     one vector: a 0-dim fp32 tensor on their device, 0 for an empty list.
 
     ``norm_type`` is 1, 2 or inf. With ``per_tensor`` the result is ``(total, norms)``, the
     second the fp32 norm of every tensor, from the same pass. ``error_if_nonfinite`` waits for
-    the result and raises ``RuntimeError`` where it is infinite or NaN."""
+    the result and raises ``RuntimeError`` where it is infinite or NaN. ``foreach`` is torch's, whose
+    implementations it chooses between: there is one here."""
     norm_type = _norm_type(norm_type)
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
@@ -80,7 +81,8 @@ def _norm_over_ranks(table, norm_type, grad_scale, max_norm, shard):
     return norm
 
 
-def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, *, grad_scale=1.0, shard=None):
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, foreach=None, *, grad_scale=1.0,
+                    shard=None):
     """Multiply the gradients of ``parameters`` in place by
     ``grad_scale * min(1, max_norm / (norm + 1e-6))``, ``norm`` being the norm of all of them
     together times ``grad_scale``; returns ``norm`` (0-dim fp32, on their device).
@@ -93,6 +95,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         error_if_nonfinite (bool): wait for the norm and raise ``RuntimeError``, the gradients
             untouched, where it is infinite or NaN. Otherwise a NaN norm makes every gradient
             NaN and an infinite one makes them 0 (NaN where they were infinite)
+        foreach: torch's choice of its implementation; there is one here
         grad_scale (float): multiplies every gradient in any case, e.g. 1 / micro-batches
         shard: the ``Sharder`` whose ``reduce_grads`` has brought each gradient to its owner.
             Collective: the norm is over all ranks' gradients, each rank scales those it owns

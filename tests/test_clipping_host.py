@@ -1,10 +1,12 @@
-"""The host's side of clipping, without a GPU: where a rank without gradients puts its state."""
+"""The host's side of clipping, without a GPU: its arguments, and where a rank without gradients puts
+its state."""
+import inspect
 import types
 
 import pytest
 import torch
 
-from muon_sr_b200 import clipping
+from muon_sr_b200 import clip_grad_norm_, clipping, get_total_norm
 from muon_sr_b200 import kernels as K
 
 
@@ -38,3 +40,17 @@ def test_rank_without_gradients_refuses_cpu_parameters():
     p.grad = torch.ones(3)
     with pytest.raises(ValueError, match="no CPU path"):
         clipping._gradients([p], types.SimpleNamespace(owned=lambda ps: []))
+
+
+def test_arguments_of_the_torch_namesakes():
+    """torch.nn.utils takes `foreach`, which chooses between its own loops."""
+    p = torch.nn.Parameter(torch.zeros(3))
+    for foreach in (None, True, False):
+        assert float(get_total_norm([], 2.0, False, foreach)) == 0.0
+        assert float(clip_grad_norm_([p], 1.0, 2.0, False, foreach)) == 0.0
+        assert float(get_total_norm([], foreach=foreach)) == 0.0
+        assert float(clip_grad_norm_([p], 1.0, foreach=foreach)) == 0.0
+    for ours, theirs in ((get_total_norm, torch.nn.utils.get_total_norm),
+                         (clip_grad_norm_, torch.nn.utils.clip_grad_norm_)):
+        names = list(inspect.signature(theirs).parameters)
+        assert list(inspect.signature(ours).parameters)[:len(names)] == names
