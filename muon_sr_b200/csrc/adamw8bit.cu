@@ -410,6 +410,7 @@ int adamw8bit_launch(const msr_adamw8bit_entry* entries, int count, const float*
                      const msr_adamw8bit_hparams* hp, const float* gscale, msr_stream_t stream) {
   if (count < 0 || (count > 0 && (entries == nullptr || hp == nullptr)))
     return fail(MSR_ERR_INVALID, "msr_adamw8bit: bad entry list or hparams");
+  if (hp == nullptr) return MSR_OK;  // no entries either
   const int bs = hp->block_size;
   if (bs < 32 || bs > 4096 || (bs & (bs - 1)))
     return fail(MSR_ERR_INVALID, "msr_adamw8bit: block_size %d is not a power of two in [32, 4096]", bs);

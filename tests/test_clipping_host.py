@@ -1,6 +1,8 @@
-"""The host's side of clipping, without a GPU: its arguments, and where a rank without gradients puts
+"""The host's side of clipping, without a GPU: arguments, refusals, and where a rank without gradients puts
 its state."""
 import inspect
+import subprocess
+import sys
 import types
 
 import pytest
@@ -8,6 +10,7 @@ import torch
 
 from muon_sr_b200 import clip_grad_norm_, clipping, get_total_norm
 from muon_sr_b200 import kernels as K
+from tests.conftest import ROOT
 
 
 class OnDevice:
@@ -54,3 +57,15 @@ def test_arguments_of_the_torch_namesakes():
                          (clip_grad_norm_, torch.nn.utils.clip_grad_norm_)):
         names = list(inspect.signature(theirs).parameters)
         assert list(inspect.signature(ours).parameters)[:len(names)] == names
+
+
+def test_8bit_launch_of_nothing_needs_no_hyperparameters():
+    """In a process of its own: the call read through the null pointer."""
+    code = ("from muon_sr_b200 import _lib; import ctypes; lib = _lib.load(); x = ctypes.create_string_buffer(64); "
+            "assert lib.msr_adamw8bit(None, 0, None, None, None, None) == 0; "
+            "assert lib.msr_adamw8bit_scaled(None, 0, None, None, None, ctypes.addressof(x) // 16 * 16 + 16, None) == 0; "
+            "assert lib.msr_adamw8bit(None, 1, None, None, None, None) == 1; "
+            "hp = _lib.Adam8Hparams(); hp.block_size = 100; "
+            "assert lib.msr_adamw8bit(None, 0, None, None, ctypes.byref(hp), None) == 1")
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert done.returncode == 0, (done.returncode, done.stderr)
