@@ -270,7 +270,7 @@ int msr_adamw8bit(const msr_adamw8bit_entry* entries, int count, const float* qm
  * double, in a fixed order: the same inputs give the same bits. NaN anywhere gives a NaN norm and
  * factor; an infinity gives norm = infinity and coef = 0.
  * msr_grad_norm writes `state` and, where `each` is given, the norm of every entry by itself
- * (scale included). The workspace is scratch of this call alone; two calls that may overlap
+ * (scale included; 4-byte aligned). The workspace is scratch of this call alone; two calls that may overlap
  * need one each.
  * msr_grad_factor computes norm, factor and active again from state->power, for a caller that
  * combined the powers of several ranks (a sum, or for infinity a maximum -- of the bit patterns

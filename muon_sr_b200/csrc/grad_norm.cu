@@ -790,6 +790,7 @@ size_t msr_grad_norm_workspace_bytes(int count) {
 
 int msr_grad_norm(const msr_grad_entry* entries, int count, int norm, double scale, double max_norm,
                   msr_clip_state* state, float* each, void* workspace, size_t workspace_bytes, msr_stream_t stream) {
+  if (reinterpret_cast<uintptr_t>(each) % 4) return fail(MSR_ERR_INVALID, "msr_grad_norm: each is not 4-byte aligned");
   if (int st = check_norm(entries, count, norm, scale, max_norm, state, workspace, workspace_bytes, "msr_grad_norm"))
     return st;
   const NormCall c{entries, count, scale, max_norm, state, each, static_cast<double*>(workspace), to_stream(stream)};

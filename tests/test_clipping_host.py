@@ -1,5 +1,6 @@
 """The host's side of clipping, without a GPU: arguments, refusals, and where a rank without gradients puts
 its state."""
+import ctypes
 import inspect
 import subprocess
 import sys
@@ -8,7 +9,7 @@ import types
 import pytest
 import torch
 
-from muon_sr_b200 import clip_grad_norm_, clipping, get_total_norm
+from muon_sr_b200 import _lib, clip_grad_norm_, clipping, get_total_norm
 from muon_sr_b200 import kernels as K
 from tests.conftest import ROOT
 
@@ -69,3 +70,14 @@ def test_8bit_launch_of_nothing_needs_no_hyperparameters():
             "assert lib.msr_adamw8bit(None, 0, None, None, ctypes.byref(hp), None) == 1")
     done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
     assert done.returncode == 0, (done.returncode, done.stderr)
+
+
+def test_norms_of_each_entry_need_an_aligned_pointer():
+    lib = _lib.load()
+    at = ctypes.create_string_buffer(64)
+    ptr = (ctypes.addressof(at) + 15) // 16 * 16      # never dereferenced: every call is refused
+    need = lib.msr_grad_norm_workspace_bytes(1)
+    entry = (ctypes.c_int64 * 3)(ptr, 4, 0)
+    for off in (1, 2, 3):
+        assert lib.msr_grad_norm(entry, 1, 2, 1.0, 1.0, ptr, ptr + 32 + off, ptr, need, None) == 1
+        assert b"each" in lib.msr_last_error()
