@@ -266,12 +266,12 @@ int msr_adamw8bit(const msr_adamw8bit_entry* entries, int count, const float* qm
  *   power  = sum |g|^p (the largest |g| for infinity);  norm = scale * power^(1/p)
  *   coef   = min(1, max_norm / (norm + 1e-6));          factor = scale * coef
  * `scale` is what the caller multiplies every gradient by in any case (1 / micro-batches, 1 /
- * loss scale); max_norm = INFINITY asks for coef = 1 whatever the norm. Sums are kept in
- * double, in a fixed order: the same inputs give the same bits. NaN anywhere gives a NaN norm and
- * factor; an infinity gives norm = infinity and coef = 0.
- * msr_grad_norm writes `state` and, where `each` is given, the norm of every entry by itself
- * (scale included; 4-byte aligned). The workspace is scratch of this call alone; two calls that may overlap
- * need one each.
+ * loss scale), a normal number of fp32; max_norm = INFINITY asks for coef = 1 whatever the norm.
+ * Sums are kept in double, in a fixed order: the same inputs give the same bits. NaN anywhere gives
+ * a NaN norm and factor; an infinity gives norm = infinity and coef = 0.
+ * msr_grad_norm writes `state` and, where `each` (4-byte aligned) is given, the norm of every entry
+ * by itself (scale included). The workspace is scratch of this call alone; two calls that may
+ * overlap need one each.
  * msr_grad_factor computes norm, factor and active again from state->power, for a caller that
  * combined the powers of several ranks (a sum, or for infinity a maximum -- of the bit patterns
  * as int64 where NaN has to survive it; powers are never negative).

@@ -26,6 +26,9 @@ from . import kernels as K
 from . import staging
 
 
+_FP32 = torch.finfo(torch.float32)
+
+
 def _norm_type(value):
     value = float(value)
     if value not in K.NORM_TYPES:
@@ -37,8 +40,8 @@ def _bounds(max_norm, grad_scale):
     max_norm, grad_scale = float(max_norm), float(grad_scale)
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
-    if not (grad_scale > 0 and math.isfinite(grad_scale)):
-        raise ValueError(f"grad_scale must be positive and finite, got {grad_scale}")
+    if not _FP32.tiny <= grad_scale <= _FP32.max:
+        raise ValueError(f"grad_scale must be positive and within the range of fp32, got {grad_scale}")
     return max_norm, grad_scale
 
 
@@ -101,7 +104,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
             Collective: the norm is over all ranks' gradients, each rank scales those it owns
 
     Gradients whose norm is within the bound are not written (``grad_scale`` 1). Two parameters
-    whose gradients share memory are refused."""
+    whose gradients share memory are refused. The factor is an fp32 number: it loses bits below
+    2^-126, where ``max_norm`` is that far below the norm."""
     norm_type = _norm_type(norm_type)
     max_norm, grad_scale = _bounds(max_norm, grad_scale)
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)

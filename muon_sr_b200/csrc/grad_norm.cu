@@ -15,6 +15,7 @@
 
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -612,7 +613,8 @@ int check_state(const msr_clip_state* state, const char* what) {
 int check_factor(int norm, double scale, double max_norm, const char* what) {
   if (norm != MSR_NORM_INF && norm != MSR_NORM_1 && norm != MSR_NORM_2)
     return fail(MSR_ERR_INVALID, "%s: unknown norm %d", what, norm);
-  if (!(scale > 0.0) || std::isinf(scale)) return fail(MSR_ERR_INVALID, "%s: scale must be positive and finite", what);
+  if (!(scale >= FLT_MIN && scale <= FLT_MAX))
+    return fail(MSR_ERR_INVALID, "%s: scale must be positive and within the range of fp32", what);
   if (!(max_norm >= 0.0)) return fail(MSR_ERR_INVALID, "%s: max_norm must be >= 0", what);
   return MSR_OK;
 }

@@ -81,3 +81,20 @@ def test_norms_of_each_entry_need_an_aligned_pointer():
     for off in (1, 2, 3):
         assert lib.msr_grad_norm(entry, 1, 2, 1.0, 1.0, ptr, ptr + 32 + off, ptr, need, None) == 1
         assert b"each" in lib.msr_last_error()
+
+
+def test_grad_scale_outside_fp32_is_refused():
+    """The factor that the kernels multiply by is fp32: beyond its range it would be 0 or infinity."""
+    p = torch.nn.Parameter(torch.zeros(3))
+    lib = _lib.load()
+    at = ctypes.create_string_buffer(64)
+    ptr = (ctypes.addressof(at) + 15) // 16 * 16      # never dereferenced: every call is refused
+    for bad in (3.5e38, 1e300, 2.0 ** -127, 1e-46, 1e-320):
+        with pytest.raises(ValueError, match="grad_scale"):
+            clip_grad_norm_([p], 1.0, grad_scale=bad)
+        with pytest.raises(ValueError, match="grad_scale"):
+            clipping.clipped_step(types.SimpleNamespace(param_groups=[]), 1.0, bad)
+        assert lib.msr_grad_factor(ptr, 2, bad, 1.0, None) == 1
+        assert b"scale" in lib.msr_last_error()
+    for good in (2.0 ** -126, 3.4e38):
+        assert float(clip_grad_norm_([p], 1.0, grad_scale=good)) == 0.0
