@@ -9,7 +9,10 @@ NVLink / NVSwitch, so the step's work is divided by the number of ranks.
   greedy on an estimated B200 time per tensor -- Newton-Schulz FLOPs at its measured
   effective rate for Muon matrices, bytes at the measured rate of each elementwise kernel.
 * Seeds and Philox counters stay global, so every rank writes exactly the bits a single GPU
-  would (Newton-Schulz computes each matrix independently of how the batch is chunked).
+  would (Newton-Schulz computes each matrix independently of how the batch is chunked). A step
+  that clips (``step(max_norm=)``) adds up the ranks' powers in double, in an order that depends
+  on the partition: its norm and factor are the same on every rank, and may differ from one GPU's
+  in the last bit of fp32.
 * Sharing: as soon as a segment of a shape stack (or a param group) is updated, its
   parameters travel from their owners (see ``transport``), so the transfers run under the
   remaining Newton-Schulz work; the step ends by waiting for all of them.
