@@ -268,7 +268,7 @@ int msr_adamw8bit(const msr_adamw8bit_entry* entries, int count, const float* qm
  * `scale` is what the caller multiplies every gradient by in any case (1 / micro-batches, 1 /
  * loss scale), a normal number of fp32; max_norm = INFINITY asks for coef = 1 whatever the norm.
  * Sums are kept in double, in a fixed order: the same inputs give the same bits. NaN anywhere gives
- * a NaN norm and factor; an infinity gives norm = infinity and coef = 0.
+ * a NaN norm, an infinity norm = infinity; with a finite max_norm the factor is then NaN or 0.
  * msr_grad_norm writes `state` and, where `each` (4-byte aligned) is given, the norm of every entry
  * by itself (scale included). The workspace is scratch of this call alone; two calls that may
  * overlap need one each.
@@ -279,8 +279,10 @@ int msr_adamw8bit(const msr_adamw8bit_entry* entries, int count, const float* qm
  * even; when state->active is 0 it leaves them untouched. Entries of one call must not share
  * memory (MSR_ERR_INVALID). An entry may start at any multiple of its element size; entries of
  * numel 0 may have a NULL pointer.
- * msr_grad_clip is msr_grad_norm followed by msr_grad_scale, in fewer launches: one for sets of
- * up to 512 KB, two otherwise (up to 512 entries). */
+ * msr_grad_clip is msr_grad_norm followed by msr_grad_scale, in fewer launches. One, where the
+ * entries make up at most 32 pieces of 16 KB, none of which spans two entries (at most 512 KB then,
+ * and at most 32 entries that are not empty); two otherwise, up to 512 entries; beyond, three for
+ * every 512 entries. msr_grad_norm takes one launch, then two for every 512 entries. */
 enum msr_dtype { MSR_BF16 = 0, MSR_FP16 = 1, MSR_FP32 = 2 };
 enum msr_norm { MSR_NORM_INF = 0, MSR_NORM_1 = 1, MSR_NORM_2 = 2 };
 

@@ -93,11 +93,13 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     Arguments:
         parameters: a parameter or an iterable of them; those without a gradient are passed
             over, one that is listed twice counts once
-        max_norm (float): the bound; ``math.inf`` clips nothing
+        max_norm (float): the bound; ``math.inf`` clips nothing, whatever the norm (torch's
+            function makes every gradient NaN where the norm is not finite)
         norm_type (float): 1, 2 or inf
         error_if_nonfinite (bool): wait for the norm and raise ``RuntimeError``, the gradients
-            untouched, where it is infinite or NaN. Otherwise a NaN norm makes every gradient
-            NaN and an infinite one makes them 0 (NaN where they were infinite)
+            untouched, where it is infinite or NaN. Otherwise, ``max_norm`` being finite, a NaN
+            norm makes every gradient NaN and an infinite gradient makes them 0 (NaN where they
+            were infinite)
         foreach: torch's choice of its implementation; there is one here
         grad_scale (float): multiplies every gradient in any case, e.g. 1 / micro-batches
         shard: the ``Sharder`` whose ``reduce_grads`` has brought each gradient to its owner.

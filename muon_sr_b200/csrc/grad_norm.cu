@@ -44,8 +44,8 @@ constexpr int GN_SCALE_BLOCKS_PER_SM = 2;
 constexpr int GN_MAX_GRID = 2048;                     // slots of the workspace besides one per tensor
 constexpr int GN_MAXE = 512;                          // tensors per launch
 constexpr int GN_FINISH_THREADS = 1024;
-// Sets of at most GN_SMALL small chunks (512 KB) are one launch of one cluster, see
-// grad_small_kernel.
+// Sets of at most GN_SMALL small chunks of 16 KB, none of which spans two tensors, are one launch of
+// one cluster, see grad_small_kernel.
 constexpr int GN_CLUSTER = 8;
 constexpr int GN_ROUNDS = 4;                          // chunks per CTA of the cluster
 constexpr int GN_SMALL = GN_CLUSTER * GN_ROUNDS;

@@ -1,11 +1,11 @@
 """Clipping on the GPU where its callers' data goes wrong: non-finite norms, gradients that
-share memory."""
+share memory, bounds of infinity, and the borders of the chunks."""
 import math
 
 import pytest
 import torch
 
-from muon_sr_b200 import TritonAdamW8bit, clip_grad_norm_
+from muon_sr_b200 import TritonAdamW8bit, clip_grad_norm_, get_total_norm
 from muon_sr_b200 import kernels as K
 
 pytestmark = pytest.mark.gpu
@@ -143,3 +143,56 @@ def test_strided_gradients_side_by_side_are_clipped(views):
     tol = scaled.abs() * (2.0 ** -8 + 37 * 2.0 ** -24) + 2.0 ** -134
     assert bool(((x.double() - scaled).abs() <= tol)[inside].all())
     assert torch.equal(x[~inside], before[~inside])
+
+
+# ---- a bound of infinity -----------------------------------------------------------------
+@pytest.mark.parametrize("sizes", [[40, 9], [9000, 600000]])  # one cluster, two kernels
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_a_bound_of_infinity_clips_nothing_whatever_the_norm(sizes, bad):
+    grads = [torch.randn(n, device=DEV).to(torch.bfloat16) for n in sizes]
+    grads[1][3] = bad
+    before = [g.clone() for g in grads]
+    norm = float(clip(grads, math.inf))
+    assert norm == math.inf if bad == math.inf else math.isnan(norm)
+    assert all(same_bits(g, b) for g, b in zip(grads, before))
+    params = [torch.nn.Parameter(torch.empty_like(g)) for g in grads]
+    for p, g in zip(params, grads):
+        p.grad = g
+    clip_grad_norm_(params, math.inf, grad_scale=0.5)                      # (exact: a power of two)
+    assert all(torch.equal(g.nan_to_num(7), (b * 0.5).nan_to_num(7)) for g, b in zip(grads, before))
+
+
+# ---- the norm at the borders of its chunks ------------------------------------------------
+# A power is a double sum of fp32 sums of at most 32 values, in two halves that are added: a term
+# passes 16 roundings (a square and its addition are one) and that of the halves, 17 * 2^-24 of a
+# sum of non-negative terms. The root halves it; the result is rounded to fp32 once more, 2^-24.
+# One more covers the products of these errors.
+TOL = {1.0: 19 * 2.0 ** -24, 2.0: (17 / 2 + 2) * 2.0 ** -24}
+
+
+@pytest.mark.parametrize("p", [1.0, 2.0])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_norm_at_chunk_borders(p, dtype, offset):
+    """Chunks are of 2048 vectors of 16 bytes (1024 in the one-cluster kernel): 16384 and 8192
+    elements of 16 and 32 bits; together these sets take the two kernels, one by one the cluster."""
+    sizes = [4095, 4096, 4097, 8191, 8192, 8193, 16383, 16384, 16385, 16391, 32767, 32768, 32769, 262143, 262144, 262145]
+    gen = torch.Generator(device=DEV).manual_seed(offset)
+    grads = [(torch.randn(offset + n, device=DEV, generator=gen) * 1e-2).to(dtype)[offset:] for n in sizes]
+    power = [float((g.double().abs() ** p).sum()) for g in grads]
+    total, each = get_total_norm(grads, p, per_tensor=True)
+    assert abs(float(total) - sum(power) ** (1 / p)) <= TOL[p] * sum(power) ** (1 / p)
+    for n, g, got, x in zip(sizes, grads, each.tolist(), power):
+        want = x ** (1 / p)
+        assert abs(got - want) <= TOL[p] * want, n
+        assert abs(float(get_total_norm([g], p)) - want) <= TOL[p] * want, n
+
+
+def test_norm_with_and_without_each():
+    """The same partial sums joined in another order: in double, so at most one fp32 step apart."""
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    grads = [torch.randn(n, device=DEV, generator=gen).to(torch.bfloat16) for n in (1000003, 5, 70001, 64, 4096 * 9)]
+    for p in (1.0, 2.0, math.inf):
+        for some in (grads, grads[1:2] + grads[3:]):
+            a, b = float(get_total_norm(some, p)), float(get_total_norm(some, p, per_tensor=True)[0])
+            assert a == b if p == math.inf else abs(a - b) <= 2.0 ** -23 * a
