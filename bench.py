@@ -851,6 +851,14 @@ def run_kernel_case(args):
             fn = lambda: K.muon_apply([(p, upd, 1.0, 7)], 0.02, 0.01)
             work = n * 6 / 1e9
         unit = "GB/s"
+    if args.scaled:  # the gradients read times a device scalar, as a step that clips reads them
+        if args.kernel not in ("adamw8bit", "adamw", "prepare"):
+            raise SystemExit("--scaled is for the kernels that read gradients: adamw8bit, adamw, prepare")
+        plain, factor = fn, torch.full((1,), 0.5, device=dev)
+
+        def fn():
+            with K.gradient_factor(factor):
+                plain()
     for _ in range(args.warmup):
         fn()
     torch.cuda.synchronize()
@@ -862,7 +870,7 @@ def run_kernel_case(args):
     torch.cuda.synchronize()
     ms = s.elapsed_time(e) / args.steps
     out.update({"ms_per_call": ms, "rate": work / (ms * 1e-3), "unit": unit, "small": bool(args.small),
-                "noise": args.noise})
+                "noise": args.noise, "scaled": bool(args.scaled)})
     print(json.dumps(out), flush=True)
 
 
@@ -880,6 +888,8 @@ def main():
                                          "grad_norm", "grad_clip"],
                     help="time one kernel alone (profiling cases) instead of the optimizer step")
     ap.add_argument("--small", action="store_true", help="with --kernel: the few-GB profiling size")
+    ap.add_argument("--scaled", action="store_true",
+                    help="with --kernel adamw8bit, adamw or prepare: gradients read times a factor (step(max_norm=))")
     ap.add_argument("--ns-shape", default=None,
                     help="with --kernel ns: the stack as BATCHxROWSxCOLS (e.g. 12x768x3072)")
     ap.add_argument("--noise", choices=["reference", "fast", "none"], default="reference",
