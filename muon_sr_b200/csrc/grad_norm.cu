@@ -578,10 +578,11 @@ int grid_for(int64_t chunks, int blocks_per_sm) {
 
 // How the scaling kernels share out the chunks. Up to a few times the L2 cache (126 MB), every
 // block takes one stretch, as in the power kernel, and begins at its end, which that kernel read
-// last: clipping 90 M bf16 elements (180 MB) takes 81 us, against 85 with groups of 2. Beyond, the
-// groups of 2 of all blocks form one window that moves through memory, which DRAM serves better:
-// clipping 1.9 G elements takes 1758 us, against 1801 by stretches.
-constexpr int64_t GN_STRETCH_BYTES = int64_t(600) << 20;
+// last. Beyond, the groups of 2 of all blocks form one window that moves through memory, which DRAM
+// serves better. Clipping 24 bf16 tensors, three sets in turn, stretches against groups in us:
+// 64 MB 35.1 / 37.3, 180 MB 92.2 / 94.4, 256 MB 132.8 / 134.0, 400 MB 207.9 / 207.3, 600 MB
+// 307 / 303, 1200 MB 601 / 585, 3840 MB 1892 / 1854.
+constexpr int64_t GN_STRETCH_BYTES = int64_t(384) << 20;
 struct ScaleShape {
   int grid;
   int64_t group;
