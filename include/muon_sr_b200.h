@@ -319,14 +319,20 @@ int msr_grad_clip(const msr_grad_entry* entries, int count, int norm, double sca
  * memory (state->factor of msr_grad_norm): the product is taken in fp32 and is not rounded to
  * bf16, and the gradients themselves stay. Everything else -- noise, order of the operations,
  * records -- is that of the call without the suffix, and grad_factor[0] = 1 gives its bits.
- * msr_adamw8bit_scaled with a grad_factor[0] that is not finite changes nothing at all: its rule for
- * non-finite gradients, resetting their moments, would reset every element's. */
+ * With a grad_factor[0] that is not finite (one NaN among all gradients) they change nothing, but
+ * for the updates of msr_muon_prepare_scaled, which become 0: stochastic rounding would make -0 of
+ * every weight and moment, and the 8-bit rule for non-finite gradients would reset every moment.
+ * msr_muon_apply_scaled is msr_muon_apply but for that: it multiplies nothing. */
 int msr_muon_prepare_scaled(const msr_prepare_entry* entries, int count, float beta, float one_minus_beta,
                             int nesterov, const float* grad_factor, msr_stream_t stream);
+int msr_muon_apply_scaled(const msr_apply_entry* entries, int count, float lr, float decay,
+                          const float* grad_factor, msr_stream_t stream);
 int msr_adamw_sr_scaled(const msr_adamw_entry* entries, int count, const msr_adamw_hparams* hp,
                         const float* grad_factor, msr_stream_t stream);
 int msr_muon_prepare_rec_scaled(const msr_prepare_entry* entries, int count, const void* record,
                                 const float* grad_factor, msr_stream_t stream);
+int msr_muon_apply_rec_scaled(const msr_apply_entry* entries, int count, const void* record,
+                              const float* grad_factor, msr_stream_t stream);
 int msr_adamw_sr_rec_scaled(const msr_adamw_entry* entries, int count, const void* record,
                             const float* grad_factor, msr_stream_t stream);
 int msr_adamw8bit_scaled(const msr_adamw8bit_entry* entries, int count, const float* qmap1,

@@ -111,6 +111,8 @@ SIGNATURES = [
     ("msr_grad_clip", c_int, [c_void_p, c_int, c_int, c_double, c_double, c_void_p, c_void_p, c_size_t, c_void_p]),
     ("msr_muon_prepare_scaled", c_int, [ctypes.POINTER(PrepareEntry), c_int, c_float, c_float, c_int, c_void_p,
                                         c_void_p]),
+    ("msr_muon_apply_scaled", c_int, [ctypes.POINTER(ApplyEntry), c_int, c_float, c_float, c_void_p, c_void_p]),
+    ("msr_muon_apply_rec_scaled", c_int, [ctypes.POINTER(ApplyEntry), c_int, c_void_p, c_void_p, c_void_p]),
     ("msr_adamw_sr_scaled", c_int, [ctypes.POINTER(AdamWEntry), c_int, ctypes.POINTER(AdamWHparams), c_void_p,
                                     c_void_p]),
     ("msr_muon_prepare_rec_scaled", c_int, [ctypes.POINTER(PrepareEntry), c_int, c_void_p, c_void_p, c_void_p]),

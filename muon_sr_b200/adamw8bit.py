@@ -86,9 +86,8 @@ class TritonAdamW8bit(Optimizer):
     these groups automatically. CUDA, dense contiguous tensors only.
 
     ``step(max_norm=, grad_scale=)`` clips the gradients by their global norm as it reads them
-    (see ``clipping``). A non-finite gradient resets its own element's moments; where it makes the
-    norm NaN, and with it the factor of every gradient, the step leaves weights and moments as they
-    were and only advances the step counters.
+    (see ``clipping``). A non-finite gradient resets its own element's moments, but not under a NaN
+    norm, by which the step changes nothing.
     """
 
     grad_norm = None  # the last step's gradient norm, where it clipped

@@ -11,9 +11,10 @@
 
 The first two take the arguments of their namesakes in ``torch.nn.utils``. Sums are kept in
 double and norms returned in fp32, whatever the gradients' type, on the device: nothing here
-waits for the GPU unless ``error_if_nonfinite`` asks for it. A step whose norm is not finite
-does what scaling by such a factor would -- except that the 8-bit AdamW step by a NaN norm leaves
-weights and moments as they were: look at ``grad_norm`` where that can happen.
+waits for the GPU unless ``error_if_nonfinite`` asks for it. A step by a NaN norm -- one NaN in
+any gradient -- leaves weights, momenta and moments as they were and only advances the step
+counters; by an infinite norm it does what gradients scaled by 0 would (NaN where they were
+infinite). ``grad_norm`` tells.
 """
 import contextlib
 import math
@@ -99,7 +100,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         error_if_nonfinite (bool): wait for the norm and raise ``RuntimeError``, the gradients
             untouched, where it is infinite or NaN. Otherwise, ``max_norm`` being finite, a NaN
             norm makes every gradient NaN and an infinite gradient makes them 0 (NaN where they
-            were infinite)
+            were infinite). Stochastic rounding carries a NaN over to -0, so a step on such
+            gradients leaves no NaN in the weights to notice it by
         foreach: torch's choice of its implementation; there is one here
         grad_scale (float): multiplies every gradient in any case, e.g. 1 / micro-batches
         shard: the ``Sharder`` whose ``reduce_grads`` has brought each gradient to its owner.

@@ -139,7 +139,7 @@ __global__ __launch_bounds__(Q_THREADS, 4) void adamw8bit_kernel(const __grid_co
   const float gs = SCALED ? *a.gscale : 1.f;
   // A factor that is not finite (one NaN among all gradients) would make every gradient so, and the
   // rule below, which resets the moments of such an element, would empty the whole optimizer:
-  // the launch leaves everything as it is instead.
+  // a launch by it changes nothing.
   if (SCALED && !finite_f(gs)) return;
   extern __shared__ __align__(16) uint8_t dsm[];
   float* q1 = reinterpret_cast<float*>(dsm);

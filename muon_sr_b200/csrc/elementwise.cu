@@ -157,6 +157,11 @@ __device__ __forceinline__ float grad_value(uint16_t bits, float gs) {
   return SCALED ? fmul(g, gs) : g;
 }
 
+// A factor that is not finite (one NaN among all gradients makes the norm so) must not reach the
+// roundings: stochastic rounding adds to the bits, and a NaN's, 0x7FFFFFFF, carry over to -0, so that
+// every weight and moment would be lost without a trace. A launch by such a factor changes nothing.
+__device__ __forceinline__ bool no_update(const float* factor) { return factor && !isfinite(*factor); }
+
 // `rnd()` yields the element's noise word; it is called after the math, where the noise is
 // consumed, which keeps the register allocation of the Philox chain as short as possible.
 template <int NOISE, bool SCALED, class Rnd>
@@ -170,9 +175,24 @@ __device__ __forceinline__ void prepare_one(uint16_t g_bits, float gs, uint16_t 
   upd_out = rne_bf16_bits(upd);
 }
 
+// The updates of a launch that leaves its momentum: what follows reads them.
+__device__ __noinline__ void zero_updates(const PrepareArgs& a) {
+  const int64_t total = a.prefix[a.count];
+  for (int64_t chunk = blockIdx.x; chunk < total; chunk += gridDim.x) {
+    const int ei = find_entry<MAXE>(a.prefix, a.count, chunk);
+    const int64_t base = (chunk - a.prefix[ei]) * EW_CHUNK;
+    const int64_t end = min(base + EW_CHUNK, a.e[ei].numel);
+    for (int64_t i = base + threadIdx.x; i < end; i += EW_THREADS) static_cast<uint16_t*>(a.e[ei].update)[i] = 0;
+  }
+}
+
 template <int NOISE, bool REC, bool SCALED>
 __global__ __launch_bounds__(EW_THREADS, 4) void muon_prepare_kernel(const __grid_constant__ PrepareArgs a) {
   constexpr bool FAST = NOISE == NOISE_FAST;
+  if (SCALED && no_update(a.gscale)) {
+    zero_updates(a);
+    return;
+  }
   const float gs = SCALED ? *a.gscale : 1.f;
   const int64_t total = a.prefix[a.count];
   const bool nesterov = (REC ? a.rec->nesterov : a.nesterov) != 0;
@@ -247,6 +267,7 @@ struct ApplyArgs {
   const msr_apply_record* rec;  // msr_muon_apply_rec (see PrepareArgs)
   int32_t src[MAXE];
   int any_mc;  // some entry stores its weights through a multicast address
+  const float* gscale;  // msr_muon_apply_scaled: the factor of the gradients behind the updates
 };
 
 template <bool REC>
@@ -290,6 +311,7 @@ __device__ __forceinline__ void apply_tail(const ApplyArgs& a, uint16_t* p, uint
 template <int NOISE, bool REC>
 __global__ __launch_bounds__(EW_THREADS, 4) void muon_apply_kernel(const __grid_constant__ ApplyArgs a) {
   constexpr bool FAST = NOISE == NOISE_FAST;
+  if (no_update(a.gscale)) return;
   const int64_t total = a.prefix[a.count];
   for (int64_t chunk = blockIdx.x; chunk < total; chunk += gridDim.x) {
     const int ei = find_entry<MAXE>(a.prefix, a.count, chunk);
@@ -423,6 +445,7 @@ __device__ __forceinline__ void adamw_tail(const AdamWArgs& a, const msr_adamw_e
 // ITERS vectors of 8 elements per thread and chunk; MINB CTAs per SM for the register budget.
 template <int ITERS, int MINB, int NOISE, bool REC, bool SCALED>
 __global__ __launch_bounds__(ADAMW_THREADS, MINB) void adamw_kernel(const __grid_constant__ AdamWArgs a) {
+  if (SCALED && no_update(a.gscale)) return;
   const float gs = SCALED ? *a.gscale : 1.f;
   constexpr int64_t CHUNK = ADAMW_THREADS * EW_VEC * ITERS;
   const int64_t total = a.prefix[a.count];
@@ -609,7 +632,7 @@ int prepare_launch(const msr_prepare_entry* entries, int count, float beta, floa
 }
 
 int apply_launch(const msr_apply_entry* entries, int count, float lr, float decay, const msr_apply_record* rec,
-                 msr_stream_t stream) {
+                 const float* gscale, msr_stream_t stream) {
   if (count < 0 || (count > 0 && entries == nullptr)) return fail(MSR_ERR_INVALID, "msr_muon_apply: bad entry list");
   int next = 0;
   while (next < count) {
@@ -617,6 +640,7 @@ int apply_launch(const msr_apply_entry* entries, int count, float lr, float deca
     a.lr = lr;
     a.decay = decay;
     a.rec = rec;
+    a.gscale = gscale;
     int64_t chunks = 0;
     int i = next;
     for (; i < count && a.count < MAXE; ++i) {
@@ -763,12 +787,12 @@ int msr_muon_prepare_rec(const msr_prepare_entry* entries, int count, const void
 }
 
 int msr_muon_apply(const msr_apply_entry* entries, int count, float lr, float decay, msr_stream_t stream) {
-  return msr::apply_launch(entries, count, lr, decay, nullptr, stream);
+  return msr::apply_launch(entries, count, lr, decay, nullptr, nullptr, stream);
 }
 
 int msr_muon_apply_rec(const msr_apply_entry* entries, int count, const void* record, msr_stream_t stream) {
   if (!msr::record_ok(record)) return fail(MSR_ERR_INVALID, "msr_muon_apply_rec: record must be 16-byte aligned");
-  return msr::apply_launch(entries, count, 0.f, 0.f, static_cast<const msr_apply_record*>(record), stream);
+  return msr::apply_launch(entries, count, 0.f, 0.f, static_cast<const msr_apply_record*>(record), nullptr, stream);
 }
 
 int msr_adamw_sr(const msr_adamw_entry* entries, int count, const msr_adamw_hparams* hp, msr_stream_t stream) {
@@ -794,6 +818,19 @@ int msr_muon_prepare_rec_scaled(const msr_prepare_entry* entries, int count, con
   if (!msr::factor_ok(grad_factor)) return fail(MSR_ERR_INVALID, "msr_muon_prepare_rec_scaled: bad grad_factor pointer");
   return msr::prepare_launch(entries, count, 0.f, 0.f, 0, static_cast<const msr_prepare_record*>(record), grad_factor,
                              stream);
+}
+
+int msr_muon_apply_scaled(const msr_apply_entry* entries, int count, float lr, float decay, const float* grad_factor,
+                          msr_stream_t stream) {
+  if (!msr::factor_ok(grad_factor)) return fail(MSR_ERR_INVALID, "msr_muon_apply_scaled: bad grad_factor pointer");
+  return msr::apply_launch(entries, count, lr, decay, nullptr, grad_factor, stream);
+}
+
+int msr_muon_apply_rec_scaled(const msr_apply_entry* entries, int count, const void* record, const float* grad_factor,
+                              msr_stream_t stream) {
+  if (!msr::record_ok(record)) return fail(MSR_ERR_INVALID, "msr_muon_apply_rec_scaled: record must be 16-byte aligned");
+  if (!msr::factor_ok(grad_factor)) return fail(MSR_ERR_INVALID, "msr_muon_apply_rec_scaled: bad grad_factor pointer");
+  return msr::apply_launch(entries, count, 0.f, 0.f, static_cast<const msr_apply_record*>(record), grad_factor, stream);
 }
 
 int msr_adamw_sr_scaled(const msr_adamw_entry* entries, int count, const msr_adamw_hparams* hp,

@@ -42,8 +42,8 @@ _SCALAR_FIELDS = {
     "msr_muon_apply_rec": ("key", "scale"),
     "msr_adamw_sr_rec": ("key_m", "key_v", "key_p", "step_size", "bc2_sqrt"),
 }
-# The launches that read their gradients times a device scalar have the same records.
-for _fn in ("msr_muon_prepare_rec", "msr_adamw_sr_rec"):
+# The launches of a step that reads its gradients times a device scalar have the same records.
+for _fn in list(_SCALAR_FIELDS):
     _SCALAR_FIELDS[_fn + "_scaled"] = _SCALAR_FIELDS[_fn]
 
 _CHANGED = ("the optimizer step no longer matches its captured graph (parameters with gradients, "

@@ -71,7 +71,7 @@ def _issuing():
 
 # ``gradient_factor(factor)``: while it is entered on this thread, the launches below that read
 # gradients (prepare, AdamW, 8-bit AdamW) multiply each by ``factor[0]``, an fp32 device tensor,
-# as they read it.
+# as they read it; where that is not finite, they and apply leave weights and state as they are.
 @contextlib.contextmanager
 def gradient_factor(factor):
     saved = _factor()
@@ -174,7 +174,12 @@ def muon_apply(items, lr: float, weight_decay: float) -> None:
     rec = _recorder()
     if rec is not None:
         hdr = _lib.ApplyRecord(float(f32(lr)), float(f32(1.0 - lr * weight_decay)), len(items), 0)
-        rec.launch("msr_muon_apply_rec", hdr, arr, dev)
+        rec.launch("msr_muon_apply_rec", hdr, arr, dev, _factor())
+        return
+    factor = _factor()
+    if factor is not None:
+        _lib.check(_lib.load().msr_muon_apply_scaled(arr, len(items), float(f32(lr)), float(f32(1.0 - lr * weight_decay)),
+                                                     factor.data_ptr(), stream_handle(dev)), "msr_muon_apply_scaled")
         return
     _lib.check(_lib.load().msr_muon_apply(arr, len(items), float(f32(lr)), float(f32(1.0 - lr * weight_decay)),
                                           stream_handle(dev)), "msr_muon_apply")

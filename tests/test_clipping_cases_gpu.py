@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from muon_sr_b200 import TritonAdamW8bit, clip_grad_norm_, get_total_norm
+from muon_sr_b200 import (MuonSRWithAuxAdam, StepGraph, TritonAdamW, TritonAdamW8bit, TritonMuonSR,
+                          TritonMuonSRWithAuxAdam, clip_grad_norm_, get_total_norm, set_sr_noise)
 from muon_sr_b200 import kernels as K
 
 pytestmark = pytest.mark.gpu
@@ -196,3 +197,115 @@ def test_norm_with_and_without_each():
         for some in (grads, grads[1:2] + grads[3:]):
             a, b = float(get_total_norm(some, p)), float(get_total_norm(some, p, per_tensor=True)[0])
             assert a == b if p == math.inf else abs(a - b) <= 2.0 ** -23 * a
+
+
+# ---- steps by a NaN norm, every optimizer -------------------------------------------------
+MUON = [(24, 40)] * 3 + [(40, 24)] * 2 + [(16, 16)]
+ADAM = [(30, 16), (16,), (4099,), (1,)]
+
+
+def hybrid(cls, params, **kw):
+    return cls([dict(params=params[:len(MUON)], use_muon=True, lr=0.02, weight_decay=0.01),
+                dict(params=params[len(MUON):], use_muon=False, lr=3e-4, eps=1e-10)], **kw)
+
+
+OPTIMIZERS = {
+    "adamw": lambda ps: TritonAdamW(ps, lr=1e-3, weight_decay=0.01),
+    "adamw centralized": lambda ps: TritonAdamW(ps, lr=1e-3, centralization=0.5),
+    "muon": lambda ps: TritonMuonSR(ps[:len(MUON)], lr=0.02, weight_decay=0.01),
+    "muon batched": lambda ps: TritonMuonSR(ps[:len(MUON)], lr=0.02, weight_decay=0.01, batch_ns=True),
+    "hybrid": lambda ps: hybrid(TritonMuonSRWithAuxAdam, ps, batch_ns=True),
+    "hybrid random": lambda ps: hybrid(MuonSRWithAuxAdam, ps, batch_ns=True),
+}
+
+
+def parameters(seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter((torch.randn(s, generator=gen) * 0.02).to(torch.bfloat16).to(DEV)) for s in MUON + ADAM]
+
+
+def refill(params, seed):
+    """New values in the gradients' memory."""
+    gen = torch.Generator().manual_seed(seed)
+    for p in params:
+        if p.grad is None:
+            p.grad = torch.empty_like(p)
+        p.grad.copy_((torch.randn(p.shape, generator=gen) * 1e-2).to(torch.bfloat16))
+
+
+@pytest.fixture(params=["reference", "fast", "none"])
+def noise(request):
+    set_sr_noise(request.param)
+    try:
+        yield request.param
+    finally:
+        set_sr_noise("reference")
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("name", OPTIMIZERS)
+def test_step_by_a_nan_norm_leaves_everything(name, offset, noise):
+    """Without that, stochastic rounding, which adds to the bits, would turn every weight and moment
+    into -0: a NaN's bits are 0x7FFFFFFF."""
+    params = parameters()
+    if offset:  # weights at odd addresses
+        for p in params:
+            p.data = torch.cat([p.data.new_zeros(offset), p.data.flatten()])[offset:].view(p.shape)
+    opt = OPTIMIZERS[name](params)
+    for step in range(2):
+        refill(params, step)
+        opt.step(max_norm=0.5)
+    before = [t.detach().clone() for t in tensors_of(params, opt)]
+    refill(params, 2)
+    params[4].grad[3, 5] = math.nan
+    for _ in range(2):
+        opt.step(max_norm=0.5)
+        assert math.isnan(float(opt.grad_norm))
+        for i, (a, b) in enumerate(zip(tensors_of(params, opt), before)):
+            assert same_bits(a, b), i
+    refill(params, 3)
+    opt.step(max_norm=0.5)
+    assert math.isfinite(float(opt.grad_norm))
+    assert all(bool(t.isfinite().all()) for t in tensors_of(params, opt))
+    assert not same_bits(params[0], before[0])
+
+
+@pytest.mark.parametrize("name", ["adamw", "muon batched", "hybrid"])
+def test_graph_of_steps_by_a_nan_norm(name):
+    params = parameters()
+    opt = OPTIMIZERS[name](params)
+    refill(params, 0)
+    opt.step(max_norm=0.5)
+    graph = StepGraph(opt, max_norm=0.5)
+    refill(params, 1)
+    graph.step()
+    before = [t.detach().clone() for t in tensors_of(params, opt)]
+    params[2].grad[0, 0] = math.nan
+    for _ in range(3):
+        graph.step()
+    assert math.isnan(float(opt.grad_norm))
+    assert all(same_bits(a, b) for a, b in zip(tensors_of(params, opt), before))
+    refill(params, 2)
+    graph.step()
+    assert math.isfinite(float(opt.grad_norm)) and not same_bits(params[0], before[0])
+
+
+def test_step_by_an_infinite_norm_is_that_of_scaled_gradients(noise):
+    """Infinity gives a factor of 0, and the damage stays where a step without clipping has it."""
+    sets = []
+    for scaled in (True, False):
+        params = parameters()
+        opt = OPTIMIZERS["hybrid"](params)
+        refill(params, 0)
+        opt.step()
+        refill(params, 1)
+        params[-2].grad[7] = math.inf
+        if scaled:
+            for p in params:
+                p.grad.mul_(0.0)
+            opt.step()
+        else:
+            opt.step(max_norm=1.0)
+            assert float(opt.grad_norm) == math.inf
+        sets.append(tensors_of(params, opt))
+    assert all(same_bits(a, b) for a, b in zip(*sets))

@@ -98,3 +98,15 @@ def test_grad_scale_outside_fp32_is_refused():
         assert b"scale" in lib.msr_last_error()
     for good in (2.0 ** -126, 3.4e38):
         assert float(clip_grad_norm_([p], 1.0, grad_scale=good)) == 0.0
+
+
+def test_scaled_apply_needs_its_factor():
+    lib = _lib.load()
+    at = ctypes.create_string_buffer(64)
+    ptr = (ctypes.addressof(at) + 15) // 16 * 16      # never dereferenced: every call is refused or empty
+    for bad in (None, ptr + 2):
+        assert lib.msr_muon_apply_scaled(None, 0, 0.02, 1.0, bad, None) == 1
+        assert lib.msr_muon_apply_rec_scaled(None, 0, ptr, bad, None) == 1
+    assert lib.msr_muon_apply_rec_scaled(None, 0, ptr + 4, ptr, None) == 1
+    assert lib.msr_muon_apply_scaled(None, 1, 0.02, 1.0, ptr, None) == 1
+    assert lib.msr_muon_apply_scaled(None, 0, 0.02, 1.0, ptr, None) == 0
